@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('B200_NVFP4_LIB') or os.path.join(_HERE, 'libb200nvfp4.so')
 _lib = None
 
-F32, BF16 = 0, 1
+F32, BF16, I8 = 0, 1, 2
 GEMV_MULTI_MAX, GEMV_M_MAX = 8, 8
 
 
@@ -27,6 +27,10 @@ class GemvJob(C.Structure):
 
 class Nvfp4Mat(C.Structure):
     _fields_ = [('packed', C.c_void_p), ('scale', C.c_void_p), ('gscale', C.c_void_p)]
+
+
+class I8RowsC(C.Structure):
+    _fields_ = [('q', C.c_void_p), ('scale', C.c_void_p)]
 
 
 class MoeLayerC(C.Structure):
@@ -81,6 +85,10 @@ def lib():
         L.b200_bf16_to_f32.argtypes = [vp, vp, st, vp]
         L.b200_nvfp4_quantize.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp]
         L.b200_nvfp4_dequantize.argtypes = [vp, C.POINTER(Nvfp4Mat), ci, ci, vp]
+        L.b200_i8_pitch.restype = st; L.b200_i8_pitch.argtypes = [ci]
+        L.b200_i8_quantize.argtypes = [vp, ci, st, ci, ci, vp, vp, vp]
+        L.b200_i8_gemm_workspace_bytes.restype = st; L.b200_i8_gemm_workspace_bytes.argtypes = [ci, ci]
+        L.b200_i8_gemm.argtypes = [vp, ci, C.POINTER(I8RowsC), vp, ci, st, ci, ci, ci, vp, vp]
         L.b200_moe_workspace_bytes.restype = st; L.b200_moe_workspace_bytes.argtypes = [C.POINTER(MoeLayerC), ci]
         L.b200_moe_route.argtypes = [vp, C.POINTER(MoeLayerC), vp, vp, vp, ci, vp]
         L.b200_moe_forward.argtypes = [vp, C.POINTER(MoeLayerC), vp, vp, vp, vp, ci, vp]
@@ -109,6 +117,7 @@ def lib():
 ENOTIMPL = 6
 EXPORTS = ['b200_nvfp4_set_byte_credit', 'b200_nvfp4_flush_byte_credit', 'b200_nvfp4_strerror', 'b200_nvfp4_version', 'b200_nvfp4_device_status', 'b200_nvfp4_selftest_bounded_wait', 'b200_nvfp4_set_option', 'b200_nvfp4_gemm', 'b200_nvfp4_gemv_multi', 'b200_nvfp4_split_workspace_bytes', 'b200_nvfp4_gemm_ws', 'b200_nvfp4_gemv_multi_ws',
            'b200_nvfp4_gemm_bf16_workspace_bytes', 'b200_nvfp4_gemm_bf16', 'b200_nvfp4_quantize_tokens', 'b200_nvfp4_gemm_bf16_exact_workspace_bytes', 'b200_nvfp4_gemm_bf16_exact', 'b200_dense_mlp_workspace_bytes', 'b200_dense_mlp', 'b200_f32_to_bf16', 'b200_bf16_to_f32', 'b200_nvfp4_quantize', 'b200_nvfp4_dequantize',
+           'b200_i8_pitch', 'b200_i8_quantize', 'b200_i8_gemm_workspace_bytes', 'b200_i8_gemm',
            'b200_moe_workspace_bytes', 'b200_moe_route', 'b200_moe_forward', 'b200_moe_experts',
            'b200_moe_forward_static', 'b200_moe_static_ws_limit', 'b200_moe_prepare', 'b200_moe_release',
            'b200_overlay_writer_open', 'b200_overlay_writer_add', 'b200_overlay_writer_close', 'b200_overlay_family',
@@ -317,6 +326,91 @@ def dequantize(W, stream=None):
     m = W.mat()
     check(lib().b200_nvfp4_dequantize(_ptr(out), C.byref(m), W.N, W.K, _stream(stream)), 'b200_nvfp4_dequantize')
     return out
+
+
+_DTYPE = {torch.float32: F32, torch.bfloat16: BF16}
+
+
+def _want(ok, what):
+    if not ok:
+        raise B200Error(what)
+
+
+def _device(*tensors):
+    """Kernels run on the current device's stream: every tensor has to lie there."""
+    for t in tensors:
+        _want(t is None or (t.is_cuda and t.get_device() == torch._C._cuda_getDevice()), 'tensors have to be on the current CUDA device')
+
+
+def _strided_rows(x, what):
+    """(dtype code, row stride) of a 2-d f32 or bf16 tensor whose rows are contiguous and do not overlap."""
+    _want(x.dim() == 2 and x.dtype in _DTYPE and x.shape[0] >= 1 and x.shape[1] >= 1, what + ' has to be a non-empty 2-d f32 or bf16 tensor')
+    M, K = x.shape
+    ld = x.stride(0) if M > 1 else K
+    _want((x.stride(1) == 1 or K == 1) and ld >= K, what + ' has to have contiguous rows')
+    return _DTYPE[x.dtype], ld
+
+
+class I8Rows:
+    """Rows of 8-bit integers, a scale per row: q int8 [rows, pitch] (pitch: K rounded up to 16), scale f32 [rows]."""
+
+    def __init__(self, q, scale, K):
+        _want(K >= 1 and q.dim() == 2 and q.dtype == torch.int8 and q.is_contiguous() and q.shape[1] == (K + 15) // 16 * 16,
+              'q has to be contiguous int8 [rows, K rounded up to 16]')
+        _want(scale.dtype == torch.float32 and scale.is_contiguous() and scale.shape == (q.shape[0],), 'scale has to be contiguous f32 [rows]')
+        _device(q, scale)
+        self.q, self.scale, self.N, self.K = q, scale, q.shape[0], K
+        self.c = I8RowsC(q.data_ptr(), scale.data_ptr())
+
+    @classmethod
+    def empty(cls, rows, K, device):
+        _want(rows >= 1 and K >= 1, 'rows and K have to be positive')
+        return cls(torch.empty((rows, (K + 15) // 16 * 16), dtype=torch.int8, device=device),
+                   torch.empty(rows, dtype=torch.float32, device=device), K)
+
+    @property
+    def nbytes(self):
+        return self.q.numel() + 4 * self.N
+
+
+def i8_quantize(x, out=None, stream=None):
+    """x [rows, K] (f32 or bf16) -> I8Rows, weights (a scale per output channel) and activations (per token) alike."""
+    dt, ld = _strided_rows(x, 'x')
+    M, K = x.shape
+    _device(x)
+    if out is None:
+        out = I8Rows.empty(M, K, x.device)
+    _want(out.N == M and out.K == K, 'out has to be I8Rows of x\'s size')
+    _device(out.q)
+    check(lib().b200_i8_quantize(_ptr(x), dt, ld, M, K, _ptr(out.q), _ptr(out.scale), _stream(stream)), 'b200_i8_quantize')
+    return out
+
+
+def i8_gemm_workspace(M, K, device):
+    """Scratch for i8_gemm on f32 or bf16 activations: their 8-bit rows."""
+    return torch.empty(lib().b200_i8_gemm_workspace_bytes(M, K), dtype=torch.uint8, device=device)
+
+
+def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
+    """y[M,N] (f32 or bf16) = x[M,K] . W^T in 8-bit integers.  W: I8Rows; x: I8Rows, or f32 / bf16 rows, which are quantised
+    within the call, into ws (i8_gemm_workspace(M, K))."""
+    if isinstance(x, I8Rows):
+        M, K, xp, dx, ld = x.N, x.K, C.addressof(x.c), I8, 0
+        _device(W.q, x.q, y)
+    else:
+        dx, ld = _strided_rows(x, 'x')
+        M, K = x.shape
+        xp = x.data_ptr()
+        if ws is None:
+            ws = i8_gemm_workspace(M, K, x.device)
+        _device(W.q, x, ws, y)
+        _want(ws.numel() * ws.element_size() >= lib().b200_i8_gemm_workspace_bytes(M, K), 'ws is too small')
+    _want(W.K == K, 'W and x have to share K')
+    if y is None:
+        y = torch.empty((M, W.N), dtype=dtype, device=W.q.device)
+    _want(y.dtype in _DTYPE and y.shape == (M, W.N) and y.is_contiguous(), 'y has to be contiguous f32 or bf16 [M, N]')
+    check(lib().b200_i8_gemm(y.data_ptr(), _DTYPE[y.dtype], C.byref(W.c), xp, dx, ld, M, W.N, K, _ptr(ws), _stream(stream)), 'b200_i8_gemm')
+    return y
 
 
 class MoeLayer:

@@ -48,6 +48,7 @@ struct GemvParams {
 // plain), written to `out` (128 bytes, host memory).  cached: remember the encoded map (weights).
 bool tmap_available();
 bool tmap_u8_2d(void* out, const void* base, size_t rows, size_t row_bytes, int box_bytes, int box_rows, bool swz, bool cached);
+bool tmap_u8_pitched(void* out, const void* base, size_t rows, size_t row_bytes, size_t pitch, int box_bytes, int box_rows, bool swz, bool cached);   // rows `pitch` bytes apart
 bool scale_box(int K, int* box, int* swz);
 
 // common.cu: byte accounting (b200_nvfp4_set_byte_credit).  credit(): host-known counts; the grouped MoE paths
@@ -119,5 +120,12 @@ __host__ __device__ inline int gx_blocks(int NT) { return (NT + 127) / 128; }
 // gemm_f16w.cu: the exact wide GEMM (weights dequantised to fp16 in the kernel, tcgen05 kind::f16).
 size_t gemm_f16w_ws_bytes(int M, int K);
 int gemm_f16w_dense(float* y, const b200_wref* W, const void* x, int x_kind, int M, int N, int K, void* ws, cudaStream_t s);
+
+// i8_rows.cu: rows of 8-bit integers, one scale per row (the rule stands there).
+constexpr int I8_MAX_K = 65536, I8_MAX_ROWS = 1 << 24;
+__host__ __device__ inline size_t i8_pitch(int K) { return ((size_t)K + 15) & ~(size_t)15; }
+int i8_quantize_launch(const void* x, int x_is_f32, size_t ldx, int rows, int K, int8_t* q, float* scale, cudaStream_t s);
+// gemm_i8.cu: y = x . W^T on tcgen05.mma kind::i8, activations already in 8 bits.
+int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows* x, int M, int N, int K, cudaStream_t s);
 
 }  // namespace b200

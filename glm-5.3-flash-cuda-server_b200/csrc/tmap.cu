@@ -28,9 +28,9 @@ static EncodeTiledFn encode_fn() {
 
 bool tmap_available() { return encode_fn() != nullptr; }
 
-static bool encode(void* out, const void* base, size_t rows, size_t row_bytes, int box_bytes, int box_rows, bool swz) {
+static bool encode(void* out, const void* base, size_t rows, size_t row_bytes, size_t pitch, int box_bytes, int box_rows, bool swz) {
     const cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+    const cuuint64_t strides[1] = {(cuuint64_t)pitch};
     const cuuint32_t box[2] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows};
     const cuuint32_t es[2] = {1, 1};
     EncodeTiledFn fn = encode_fn();
@@ -40,7 +40,7 @@ static bool encode(void* out, const void* base, size_t rows, size_t row_bytes, i
 }
 
 namespace {
-struct Key { const void* base; size_t rows, row_bytes; int box_bytes, box_rows, swz, used; };
+struct Key { const void* base; size_t rows, row_bytes, pitch; int box_bytes, box_rows, swz, used; };
 struct Entry { Key k; alignas(64) unsigned char map[128]; };
 constexpr int CACHE_SLOTS = 2048;
 Entry g_cache[CACHE_SLOTS];
@@ -48,19 +48,23 @@ std::mutex g_cache_mu;
 }  // namespace
 
 bool tmap_u8_2d(void* out, const void* base, size_t rows, size_t row_bytes, int box_bytes, int box_rows, bool swz, bool cached) {
+    return tmap_u8_pitched(out, base, rows, row_bytes, row_bytes, box_bytes, box_rows, swz, cached);
+}
+
+bool tmap_u8_pitched(void* out, const void* base, size_t rows, size_t row_bytes, size_t pitch, int box_bytes, int box_rows, bool swz, bool cached) {
     static_assert(sizeof(CUtensorMap) == 128, "tensor map size");
-    if (!cached) return encode(out, base, rows, row_bytes, box_bytes, box_rows, swz);
+    if (!cached) return encode(out, base, rows, row_bytes, pitch, box_bytes, box_rows, swz);
     size_t h = (size_t)((uintptr_t)base >> 4) * 0x9E3779B97F4A7C15ull;
     h ^= (rows * 1315423911u) ^ (row_bytes << 7) ^ ((size_t)box_rows << 20) ^ ((size_t)box_bytes << 3) ^ (size_t)swz;
     Entry& e = g_cache[(h >> 17) % CACHE_SLOTS];
     std::lock_guard<std::mutex> lk(g_cache_mu);
-    if (e.k.used && e.k.base == base && e.k.rows == rows && e.k.row_bytes == row_bytes && e.k.box_bytes == box_bytes &&
-        e.k.box_rows == box_rows && e.k.swz == (int)swz) {
+    if (e.k.used && e.k.base == base && e.k.rows == rows && e.k.row_bytes == row_bytes && e.k.pitch == pitch &&
+        e.k.box_bytes == box_bytes && e.k.box_rows == box_rows && e.k.swz == (int)swz) {
         memcpy(out, e.map, 128);
         return true;
     }
-    if (!encode(e.map, base, rows, row_bytes, box_bytes, box_rows, swz)) { e.k.used = 0; return false; }
-    e.k = Key{base, rows, row_bytes, box_bytes, box_rows, (int)swz, 1};
+    if (!encode(e.map, base, rows, row_bytes, pitch, box_bytes, box_rows, swz)) { e.k.used = 0; return false; }
+    e.k = Key{base, rows, row_bytes, pitch, box_bytes, box_rows, (int)swz, 1};
     memcpy(out, e.map, 128);
     return true;
 }

@@ -39,6 +39,7 @@ enum {
     B200_ECOMM = 8        /* NCCL is missing or returned an error */
 };
 enum { B200_F32 = 0, B200_BF16 = 1 };          /* dtype of a non-quantised weight (gemv.h:13) */
+enum { B200_I8 = 2 };                          /* activations given as b200_i8_rows (b200_i8_gemm) */
 enum { B200_GEMV_MULTI_MAX = 8, B200_GEMV_M_MAX = 8 };
 
 /* Weight handle.  Mirrors glm5::WRef (reference include/gemv.h:16-26): a plain row-major
@@ -212,6 +213,37 @@ int b200_nvfp4_quantize_tokens(const void* x, int x_is_f32, int M, int K, uint8_
 size_t b200_dense_mlp_workspace_bytes(int M, int hidden, int inter);
 int b200_dense_mlp(const float* x, const b200_wref* gate, const b200_wref* up, const b200_wref* down,
                    int hidden, int inter, float limit, float* y, void* ws, int M, b200_stream stream);
+
+/* ---- 8-bit integers: a scale per row -----------------------------------------------------------------
+ * The second weight format of the library, for matrices whose 4-bit error is too large: half the bytes of bf16, about 1 %
+ * from the unquantised product, and exact from there on.  A matrix is brought to rows of whole numbers -127 .. 127 with one
+ * f32 scale per row by one rule, weights [N, K] once (a scale per output channel) and activations [M, K] per call (a scale per
+ * token); every step is one f32 operation, so that any implementation of the rule gives the same codes:
+ *   a = max(max |x[r, :]|, 2^-119)    scale[r] = a / 127    q[r, k] = round_half_to_even(x[r, k] * (127 / a))
+ * A row that holds an infinity or a NaN gets a NaN scale and codes of zero, so that its products are NaN.
+ * Rows are b200_i8_pitch(K) bytes apart (K rounded up to 16); the bytes past K are written as zero and never used.
+ * No counterpart in the reference. */
+typedef struct {
+    const int8_t* q;          /* [rows, b200_i8_pitch(K)], 16-byte aligned */
+    const float*  scale;      /* [rows] */
+} b200_i8_rows;
+size_t b200_i8_pitch(int K);
+
+/* x [rows, K] (dtype B200_F32 or B200_BF16, rows ldx >= K elements apart, at its type's alignment; 16-byte aligned rows are
+ * fastest) -> q, scale.  K <= 65536, rows <= 2^24 (B200_ELIMIT). */
+int b200_i8_quantize(const void* x, int dtype, size_t ldx, int rows, int K, int8_t* q, float* scale, b200_stream stream);
+
+/* y[m, n] = x_scale[m] * W.scale[n] * sum_k xq[m, k] * W.q[n, k], y [M, N] row-major f32 (y_dtype B200_F32) or bf16.
+ * The sum is exact in 32 bits; it is rounded to f32 and multiplied by x_scale[m], then by W.scale[n], each rounded to f32, and
+ * for bf16 rounded once more.  A result does not depend on the other rows of the batch, on M, or on the run.
+ * x_dtype B200_F32 / B200_BF16: x [M, K] with rows ldx elements apart, quantised inside the call by the rule above, into ws
+ *   (b200_i8_gemm_workspace_bytes(M, K) bytes of device memory, 256-byte aligned, used only by this call's kernels).
+ * x_dtype B200_I8: x is a HOST pointer to the b200_i8_rows of the activations (b200_i8_quantize: once for several products that
+ *   share them); ldx and ws are not used.
+ * Any M, N >= 1 (<= 2^24) and 1 <= K <= 65536.  No counterpart in the reference, whose formats are NVFP4, bf16 and f32. */
+size_t b200_i8_gemm_workspace_bytes(int M, int K);
+int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const void* x, int x_dtype, size_t ldx, int M, int N, int K,
+                 void* ws, b200_stream stream);
 
 /* Element-wise converters (reference include/gemv.h:61-62, kernels/gemv.cu:470-488). */
 int b200_f32_to_bf16(void* dst_bf16, const float* src, size_t n, b200_stream stream);

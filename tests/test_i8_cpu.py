@@ -1,0 +1,67 @@
+"""8-bit products: what the entry points refuse on the host, before any CUDA call."""
+import ctypes as C
+
+import pytest
+import torch
+
+from util import pkg
+
+OK, EINVAL, EALIGN, ELIMIT = 0, 1, 3, 5
+PTR = 1 << 20                                               # an address that is never read
+
+
+def test_pitch_and_workspace():
+    L = pkg().lib()
+    assert [L.b200_i8_pitch(k) for k in (-1, 0, 1, 16, 17, 4096)] == [0, 0, 16, 16, 32, 4096]
+    for M, K in ((1, 1), (5, 2051), (2048, 4096)):
+        n = L.b200_i8_gemm_workspace_bytes(M, K)
+        assert n % 256 == 0 and n >= M * ((K + 15) // 16 * 16 + 4)
+    assert L.b200_i8_gemm_workspace_bytes(1 << 24, 65536) > 1 << 40      # no 32-bit product
+
+
+@pytest.mark.parametrize('change,code', [
+    (dict(x=None), EINVAL), (dict(q=None), EINVAL), (dict(scale=None), EINVAL), (dict(dtype=2), EINVAL), (dict(dtype=-1), EINVAL),
+    (dict(ldx=63), EINVAL), (dict(rows=0), EINVAL), (dict(rows=-1), EINVAL), (dict(K=0), EINVAL), (dict(K=65537, ldx=65537), ELIMIT),
+    (dict(rows=(1 << 24) + 1), ELIMIT), (dict(x=PTR + 2), EALIGN), (dict(x=PTR + 1, dtype=1), EALIGN), (dict(q=PTR + 8), EALIGN),
+    (dict(scale=PTR + 2), EALIGN)])
+def test_quantize_refuses(change, code):
+    a = dict(x=PTR, dtype=0, ldx=64, rows=4, K=64, q=PTR, scale=PTR)
+    a.update(change)
+    assert pkg().lib().b200_i8_quantize(a['x'], a['dtype'], a['ldx'], a['rows'], a['K'], a['q'], a['scale'], None) == code
+
+
+@pytest.mark.parametrize('change,code', [
+    (dict(y=None), EINVAL), (dict(x=None), EINVAL), (dict(wq=None), EINVAL), (dict(ws_=None), EINVAL), (dict(ws=None), EINVAL),
+    (dict(M=0), EINVAL), (dict(N=0), EINVAL), (dict(K=0), EINVAL), (dict(yd=2), EINVAL), (dict(xd=3), EINVAL), (dict(ldx=63), EINVAL),
+    (dict(M=(1 << 24) + 1), ELIMIT), (dict(N=(1 << 24) + 1), ELIMIT), (dict(K=65537, ldx=65537), ELIMIT),
+    (dict(y=PTR + 2), EALIGN), (dict(y=PTR + 1, yd=1), EALIGN), (dict(wq=PTR + 8), EALIGN), (dict(ws_=PTR + 1), EALIGN), (dict(ws=PTR + 128), EALIGN),
+    (dict(x=PTR + 2), EALIGN)])
+def test_gemm_refuses(change, code):
+    P = pkg()
+    a = dict(y=PTR, yd=0, wq=PTR, ws_=PTR, x=PTR, xd=0, ldx=64, M=4, N=8, K=64, ws=PTR)
+    a.update(change)
+    W = P.I8RowsC(a['wq'], a['ws_'])
+    assert P.lib().b200_i8_gemm(a['y'], a['yd'], C.byref(W), a['x'], a['xd'], a['ldx'], a['M'], a['N'], a['K'], a['ws'], None) == code
+
+
+@pytest.mark.parametrize('q,scale,code', [(None, PTR, EINVAL), (PTR, None, EINVAL), (PTR + 4, PTR, EALIGN), (PTR, PTR + 3, EALIGN)])
+def test_gemm_refuses_rows(q, scale, code):
+    P = pkg()
+    W, x = P.I8RowsC(PTR, PTR), P.I8RowsC(q, scale)
+    assert P.lib().b200_i8_gemm(PTR, 0, C.byref(W), C.addressof(x), P.I8, 0, 4, 8, 64, None, None) == code
+
+
+def test_binding_refuses():
+    P = pkg()
+    for bad in (torch.zeros(4), torch.zeros(2, 3, 4), torch.zeros(4, 8, dtype=torch.float16), torch.zeros(8, 4).T, torch.zeros(1, 8).expand(4, 8),
+                torch.zeros(0, 8), torch.zeros(4, 0), torch.zeros(4, 16)[:, ::2]):
+        with pytest.raises(P.B200Error):
+            P.i8_quantize(bad)
+    with pytest.raises(P.B200Error, match='current CUDA device'):
+        P.i8_quantize(torch.zeros(4, 8))
+    with pytest.raises(P.B200Error):
+        P.I8Rows(torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4), 8)             # rows are 16 bytes apart
+    with pytest.raises(P.B200Error):
+        P.I8Rows(torch.zeros(4, 16, dtype=torch.int8), torch.zeros(5), 8)
+    with pytest.raises(P.B200Error):
+        P.I8Rows.empty(0, 8, 'cpu')
