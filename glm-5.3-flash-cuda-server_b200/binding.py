@@ -89,6 +89,7 @@ def lib():
         L.b200_i8_quantize.argtypes = [vp, ci, st, ci, ci, vp, vp, vp]
         L.b200_i8_gemm_workspace_bytes.restype = st; L.b200_i8_gemm_workspace_bytes.argtypes = [ci, ci]
         L.b200_i8_gemm.argtypes = [vp, ci, C.POINTER(I8RowsC), vp, ci, st, ci, ci, ci, vp, vp]
+        L.b200_token_logprobs.argtypes = [vp, ci, st, ci, ci, vp, ci, vp, vp, ci, vp, vp, vp]
         L.b200_moe_workspace_bytes.restype = st; L.b200_moe_workspace_bytes.argtypes = [C.POINTER(MoeLayerC), ci]
         L.b200_moe_route.argtypes = [vp, C.POINTER(MoeLayerC), vp, vp, vp, ci, vp]
         L.b200_moe_forward.argtypes = [vp, C.POINTER(MoeLayerC), vp, vp, vp, vp, ci, vp]
@@ -117,7 +118,7 @@ def lib():
 ENOTIMPL = 6
 EXPORTS = ['b200_nvfp4_set_byte_credit', 'b200_nvfp4_flush_byte_credit', 'b200_nvfp4_strerror', 'b200_nvfp4_version', 'b200_nvfp4_device_status', 'b200_nvfp4_selftest_bounded_wait', 'b200_nvfp4_set_option', 'b200_nvfp4_gemm', 'b200_nvfp4_gemv_multi', 'b200_nvfp4_split_workspace_bytes', 'b200_nvfp4_gemm_ws', 'b200_nvfp4_gemv_multi_ws',
            'b200_nvfp4_gemm_bf16_workspace_bytes', 'b200_nvfp4_gemm_bf16', 'b200_nvfp4_quantize_tokens', 'b200_nvfp4_gemm_bf16_exact_workspace_bytes', 'b200_nvfp4_gemm_bf16_exact', 'b200_dense_mlp_workspace_bytes', 'b200_dense_mlp', 'b200_f32_to_bf16', 'b200_bf16_to_f32', 'b200_nvfp4_quantize', 'b200_nvfp4_dequantize',
-           'b200_i8_pitch', 'b200_i8_quantize', 'b200_i8_gemm_workspace_bytes', 'b200_i8_gemm',
+           'b200_i8_pitch', 'b200_i8_quantize', 'b200_i8_gemm_workspace_bytes', 'b200_i8_gemm', 'b200_token_logprobs',
            'b200_moe_workspace_bytes', 'b200_moe_route', 'b200_moe_forward', 'b200_moe_experts',
            'b200_moe_forward_static', 'b200_moe_static_ws_limit', 'b200_moe_prepare', 'b200_moe_release',
            'b200_overlay_writer_open', 'b200_overlay_writer_add', 'b200_overlay_writer_close', 'b200_overlay_family',
@@ -411,6 +412,35 @@ def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
     _want(y.dtype in _DTYPE and y.shape == (M, W.N) and y.is_contiguous(), 'y has to be contiguous f32 or bf16 [M, N]')
     check(lib().b200_i8_gemm(y.data_ptr(), _DTYPE[y.dtype], C.byref(W.c), xp, dx, ld, M, W.N, K, _ptr(ws), _stream(stream)), 'b200_i8_gemm')
     return y
+
+
+LOGPROBS_TOP_MAX = 32
+
+
+def token_logprobs_out(tokens, top):
+    """Output buffers of token_logprobs for these tokens."""
+    M, dev = tokens.shape[0], tokens.device
+    return (torch.empty(tokens.shape, dtype=torch.float32, device=dev), torch.empty(M, dtype=torch.float32, device=dev),
+            torch.empty((M, top), dtype=torch.int32, device=dev), torch.empty((M, top), dtype=torch.float32, device=dev))
+
+
+def token_logprobs(logits, tokens, top=0, out=None, stream=None):
+    """ln p of the given tokens (tokens int32 [M, G]; negative: none, 0), the entropy in nats, and the `top` likeliest tokens of every
+    row of logits [M, V] (f32 or bf16): (logprobs [M, G], entropy [M], top_ids [M, top], top_logprobs [M, top])."""
+    dt, ld = _strided_rows(logits, 'logits')
+    M, V = logits.shape
+    _want(tokens.dim() == 2 and tokens.shape[0] == M and tokens.dtype == torch.int32 and tokens.is_contiguous(), 'tokens has to be contiguous int32 [M, G]')
+    G = tokens.shape[1]
+    if out is None:
+        out = token_logprobs_out(tokens, top)
+    else:
+        for t, shape, dtype in zip(out, ((M, G), (M,), (M, top), (M, top)), (torch.float32, torch.float32, torch.int32, torch.float32)):
+            _want(t.shape == shape and t.dtype == dtype and t.is_contiguous(), 'out has to be token_logprobs_out(tokens, top)')
+    lp, ent, ids, tlp = out
+    _device(logits, tokens, lp, ent, ids, tlp)
+    check(lib().b200_token_logprobs(_ptr(logits), dt, ld, M, V, _ptr(tokens), G, _ptr(lp), _ptr(ent), top, _ptr(ids), _ptr(tlp), _stream(stream)),
+          'b200_token_logprobs')
+    return lp, ent, ids, tlp
 
 
 class MoeLayer:

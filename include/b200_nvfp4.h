@@ -245,6 +245,22 @@ size_t b200_i8_gemm_workspace_bytes(int M, int K);
 int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const void* x, int x_dtype, size_t ldx, int M, int N, int K,
                  void* ws, b200_stream stream);
 
+/* What a scorer reads off the vocabulary projection, in one pass over the logits [M, V] (dtype B200_F32 or B200_BF16, rows ld >= V
+ * elements apart, at their type's alignment), with p = softmax(row):
+ *   logprobs [M, G] f32   ln p of the row's G given tokens (tokens [M, G] int32).  A negative token stands for none: 0.
+ *                         One that is V or more: NaN.
+ *   entropy [M] f32       -sum p ln p, in nats
+ *   top_ids [M, top] int32, top_logprobs [M, top] f32   the `top` likeliest tokens, descending, ties to the lower index
+ * G = 0 and top = 0 leave those outputs out (their pointers are not used).  top <= min(V, B200_LOGPROBS_TOP_MAX).
+ * Masked tokens have logit -inf (ln p = -inf) or the type's lowest value.  A row of -inf alone has no distribution: its log
+ * probabilities are -inf, its entropy 0, its ids the lowest.  A row that holds +inf or a NaN: NaN, and ids of -1 (a negative
+ * token still gives 0).  Sums are held in f32, and the likeliest token's share apart from the others', so that ln p of a nearly certain token keeps its
+ * relative precision.  The same call gives the same bits.  No workspace.  V <= 2^30, M <= 2^24 (B200_ELIMIT).
+ * The reference copies the logits to the host for each token (src/engine.cu:706) and has no counterpart. */
+enum { B200_LOGPROBS_TOP_MAX = 32 };
+int b200_token_logprobs(const void* logits, int dtype, size_t ld, int M, int V, const int32_t* tokens, int G, float* logprobs,
+                        float* entropy, int top, int32_t* top_ids, float* top_logprobs, b200_stream stream);
+
 /* Element-wise converters (reference include/gemv.h:61-62, kernels/gemv.cu:470-488). */
 int b200_f32_to_bf16(void* dst_bf16, const float* src, size_t n, b200_stream stream);
 int b200_bf16_to_f32(float* dst, const void* src_bf16, size_t n, b200_stream stream);
