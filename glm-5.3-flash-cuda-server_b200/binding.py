@@ -340,16 +340,28 @@ def _want(ok, what):
 def _device(*tensors):
     """Kernels run on the current device's stream: every tensor has to lie there."""
     for t in tensors:
-        _want(t is None or (t.is_cuda and t.get_device() == torch._C._cuda_getDevice()), 'tensors have to be on the current CUDA device')
+        if not t.is_cuda:
+            raise B200Error('tensors have to be on the current CUDA device')
+    dev = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t.get_device() != dev:
+            raise B200Error('tensors have to be on the current CUDA device')
 
 
 def _strided_rows(x, what):
-    """(dtype code, row stride) of a 2-d f32 or bf16 tensor whose rows are contiguous and do not overlap."""
-    _want(x.dim() == 2 and x.dtype in _DTYPE and x.shape[0] >= 1 and x.shape[1] >= 1, what + ' has to be a non-empty 2-d f32 or bf16 tensor')
-    M, K = x.shape
-    ld = x.stride(0) if M > 1 else K
-    _want((x.stride(1) == 1 or K == 1) and ld >= K, what + ' has to have contiguous rows')
-    return _DTYPE[x.dtype], ld
+    """(dtype code, rows, columns, row stride) of a 2-d f32 or bf16 tensor whose rows are contiguous and do not overlap."""
+    dt, shape = _DTYPE.get(x.dtype), x.shape
+    if dt is None or len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
+        raise B200Error(what + ' has to be a non-empty 2-d f32 or bf16 tensor')
+    M, K = shape
+    if x.is_contiguous():
+        return dt, M, K, K
+    ld, one = x.stride()
+    if M == 1:
+        ld = K
+    if (one != 1 and K != 1) or ld < K:
+        raise B200Error(what + ' has to have contiguous rows')
+    return dt, M, K, ld
 
 
 class I8Rows:
@@ -362,6 +374,7 @@ class I8Rows:
         _device(q, scale)
         self.q, self.scale, self.N, self.K = q, scale, q.shape[0], K
         self.c = I8RowsC(q.data_ptr(), scale.data_ptr())
+        self.ref, self.addr = C.byref(self.c), C.addressof(self.c)
 
     @classmethod
     def empty(cls, rows, K, device):
@@ -376,14 +389,14 @@ class I8Rows:
 
 def i8_quantize(x, out=None, stream=None):
     """x [rows, K] (f32 or bf16) -> I8Rows, weights (a scale per output channel) and activations (per token) alike."""
-    dt, ld = _strided_rows(x, 'x')
-    M, K = x.shape
-    _device(x)
+    dt, M, K, ld = _strided_rows(x, 'x')
     if out is None:
+        _device(x)
         out = I8Rows.empty(M, K, x.device)
-    _want(out.N == M and out.K == K, 'out has to be I8Rows of x\'s size')
-    _device(out.q)
-    check(lib().b200_i8_quantize(_ptr(x), dt, ld, M, K, _ptr(out.q), _ptr(out.scale), _stream(stream)), 'b200_i8_quantize')
+    if out.N != M or out.K != K:
+        raise B200Error('out has to be I8Rows of the size of x')
+    _device(x, out.q)
+    check(lib().b200_i8_quantize(x.data_ptr(), dt, ld, M, K, out.c.q, out.c.scale, _stream(stream)), 'b200_i8_quantize')
     return out
 
 
@@ -396,21 +409,26 @@ def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
     """y[M,N] (f32 or bf16) = x[M,K] . W^T in 8-bit integers.  W: I8Rows; x: I8Rows, or f32 / bf16 rows, which are quantised
     within the call, into ws (i8_gemm_workspace(M, K))."""
     if isinstance(x, I8Rows):
-        M, K, xp, dx, ld = x.N, x.K, C.addressof(x.c), I8, 0
-        _device(W.q, x.q, y)
+        M, K, xp, dx, ld, xt, ws, wp = x.N, x.K, x.addr, I8, 0, x.q, x.q, None      # x itself holds what xp points to: it stays bound
     else:
-        dx, ld = _strided_rows(x, 'x')
-        M, K = x.shape
-        xp = x.data_ptr()
+        dx, M, K, ld = _strided_rows(x, 'x')
+        xt, xp = x, x.data_ptr()
         if ws is None:
             ws = i8_gemm_workspace(M, K, x.device)
-        _device(W.q, x, ws, y)
-        _want(ws.numel() * ws.element_size() >= lib().b200_i8_gemm_workspace_bytes(M, K), 'ws is too small')
-    _want(W.K == K, 'W and x have to share K')
+        if ws.nbytes < (M * ((K + 15) & ~15) + 255 & ~255) + (4 * M + 255 & ~255):
+            raise B200Error('ws is smaller than i8_gemm_workspace(M, K)')
+        wp = ws.data_ptr()
+    if W.K != K:
+        raise B200Error('W and x have to share K')
     if y is None:
         y = torch.empty((M, W.N), dtype=dtype, device=W.q.device)
-    _want(y.dtype in _DTYPE and y.shape == (M, W.N) and y.is_contiguous(), 'y has to be contiguous f32 or bf16 [M, N]')
-    check(lib().b200_i8_gemm(y.data_ptr(), _DTYPE[y.dtype], C.byref(W.c), xp, dx, ld, M, W.N, K, _ptr(ws), _stream(stream)), 'b200_i8_gemm')
+    dy = _DTYPE.get(y.dtype)
+    if dy is None or y.shape != (M, W.N) or not y.is_contiguous():
+        raise B200Error('y has to be contiguous f32 or bf16 [M, N]')
+    _device(W.q, xt, ws, y)
+    rc = lib().b200_i8_gemm(y.data_ptr(), dy, W.ref, xp, dx, ld, M, W.N, K, wp, _stream(stream))
+    if rc:
+        check(rc, 'b200_i8_gemm')
     return y
 
 
@@ -427,19 +445,23 @@ def token_logprobs_out(tokens, top):
 def token_logprobs(logits, tokens, top=0, out=None, stream=None):
     """ln p of the given tokens (tokens int32 [M, G]; negative: none, 0), the entropy in nats, and the `top` likeliest tokens of every
     row of logits [M, V] (f32 or bf16): (logprobs [M, G], entropy [M], top_ids [M, top], top_logprobs [M, top])."""
-    dt, ld = _strided_rows(logits, 'logits')
-    M, V = logits.shape
-    _want(tokens.dim() == 2 and tokens.shape[0] == M and tokens.dtype == torch.int32 and tokens.is_contiguous(), 'tokens has to be contiguous int32 [M, G]')
+    dt, M, V, ld = _strided_rows(logits, 'logits')
+    if tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != M or not tokens.is_contiguous():
+        raise B200Error('tokens has to be contiguous int32 [M, G]')
     G = tokens.shape[1]
     if out is None:
+        _want(top >= 0, 'top may not be negative')
         out = token_logprobs_out(tokens, top)
-    else:
-        for t, shape, dtype in zip(out, ((M, G), (M,), (M, top), (M, top)), (torch.float32, torch.float32, torch.int32, torch.float32)):
-            _want(t.shape == shape and t.dtype == dtype and t.is_contiguous(), 'out has to be token_logprobs_out(tokens, top)')
     lp, ent, ids, tlp = out
+    if (lp.shape != (M, G) or ent.shape != (M,) or ids.shape != (M, top) or tlp.shape != (M, top) or ids.dtype != torch.int32 or
+            not (lp.dtype == ent.dtype == tlp.dtype == torch.float32) or
+            not (lp.is_contiguous() and ent.is_contiguous() and ids.is_contiguous() and tlp.is_contiguous())):
+        raise B200Error('out has to be token_logprobs_out(tokens, top)')
     _device(logits, tokens, lp, ent, ids, tlp)
-    check(lib().b200_token_logprobs(_ptr(logits), dt, ld, M, V, _ptr(tokens), G, _ptr(lp), _ptr(ent), top, _ptr(ids), _ptr(tlp), _stream(stream)),
-          'b200_token_logprobs')
+    rc = lib().b200_token_logprobs(logits.data_ptr(), dt, ld, M, V, tokens.data_ptr(), G, lp.data_ptr(), ent.data_ptr(), top, ids.data_ptr(),
+                                   tlp.data_ptr(), _stream(stream))
+    if rc:
+        check(rc, 'b200_token_logprobs')
     return lp, ent, ids, tlp
 
 

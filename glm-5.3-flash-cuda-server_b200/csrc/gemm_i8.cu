@@ -11,39 +11,51 @@
 //   warp 1      MMA issuer: four tcgen05.mma (K = 32 each) per step; tcgen05.commit frees the stage
 //   warp 2      allocates / frees TMEM
 //   warps 4-11  epilogue: two groups of four warps (one per TMEM lane quadrant) take alternate 16-token chunks
+// Where the items would leave SMs idle, a cluster of CTAs shares one item (SPLIT): each takes a part of K, leaves its sums in its own
+// shared memory, and adds and writes its share of the tokens over distributed shared memory; two CTAs per SM.
 // Rows past N or M and columns past K come as zero from the tensor maps.  Every wait is bounded (tma_pipe.cuh).
 #include "b200_internal.h"
 #include "umma_mxf4.cuh"
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cooperative_groups.h>
 
 namespace b200 {
+namespace cg = cooperative_groups;
 
 constexpr int GI_THREADS = 384;
 constexpr int GI_MAX_STAGES = 12;
-constexpr int GI_TMEM_COLS = 512;
+constexpr int GI_MAX_NT = 256, GI_MAX_SPLIT = 8;
+constexpr uint32_t GI_A_BYTES = 16384;
+constexpr size_t GI_STATIC = 4096;                 // static shared memory, at most
+constexpr size_t GI_SMEM = 227 * 1024 - GI_STATIC, GI_SMEM_SPLIT = 113 * 1024 - GI_STATIC;
 
 struct GiParams {
     void* y; const float* sw; const float* sx; unsigned int* status;
-    int M, N, nst, n_jobs, total, stages;
+    int M, N, nst, NT, n_jobs, total, stages, split, tmem_cols;
 };
 
-template <int NT, bool BF16>
-__global__ void __launch_bounds__(GI_THREADS, 1)
+__device__ __forceinline__ void gi_store(void* y, size_t o, int acc, float sx, float sw, bool bf16) {
+    const float v = __fmul_rn(__fmul_rn(__int2float_rn(acc), sx), sw);
+    if (bf16) static_cast<__nv_bfloat16*>(y)[o] = __float2bfloat16_rn(v);
+    else static_cast<float*>(y)[o] = v;
+}
+
+template <bool BF16, bool SPLIT>
+__global__ void __launch_bounds__(GI_THREADS, SPLIT ? 2 : 1)
 k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
-    constexpr uint32_t A_BYTES = 16384, B_BYTES = NT * 128u, SLOT = A_BYTES + B_BYTES;
-    static_assert(SLOT % 1024 == 0, "swizzled operands start on 1024-byte boundaries");
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ uint64_t full_bar[GI_MAX_STAGES], empty_bar[GI_MAX_STAGES], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_base_s;
-    __shared__ float sxs[2][NT];
+    __shared__ float sxs[2][GI_MAX_NT];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int nst = p.nst, S = p.stages;
+    const int S = p.stages, NT = p.NT;
+    const uint32_t slot = GI_A_BYTES + (uint32_t)NT * 128u;
     // TMEM is taken after the kernel before has ended and before the kernel after may start: a kernel that held the columns
     // while it waits for another that wants them on the same SM would wait for good.
     pdl_wait();
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_base_s)), "r"(GI_TMEM_COLS));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_base_s)), "r"(p.tmem_cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     } else if (warp == 1) {
         if (lane < S) { mbar_init(smem_u32(&full_bar[lane]), 1); mbar_init(smem_u32(&empty_bar[lane]), 1); }
@@ -55,9 +67,12 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
     gx_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem = tmem_base_s;
-    const int first = blockIdx.x, stride = gridDim.x;
+    // SPLIT: one item per cluster, this CTA's part of its K steps; otherwise every gridDim-th item, all of its steps
+    const int rank = SPLIT ? (int)cg::this_cluster().block_rank() : 0;
+    const int first = SPLIT ? (int)blockIdx.x / p.split : (int)blockIdx.x, stride = SPLIT ? p.total : (int)gridDim.x;
+    const int k_first = SPLIT ? p.nst * rank / p.split : 0, nst = SPLIT ? p.nst * (rank + 1) / p.split - k_first : p.nst;
     const int n_items = (p.total - first + stride - 1) / stride;      // the grid is no larger than the number of items
-    const uint32_t ring0 = smem_u32(smem) + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
+    const uint32_t pad = (1024u - (smem_u32(smem) & 1023u)) & 1023u, ring0 = smem_u32(smem) + pad;
     const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]);
 
     if (warp == 0) {
@@ -67,10 +82,10 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
             for (int it = 0; it < nst; ++it) {
                 mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
                 if (elect_one()) {
-                    const uint32_t bar = full0 + s * 8, dst = ring0 + (uint32_t)s * SLOT;
-                    mbar_expect_tx(bar, SLOT);
-                    gx_tma_2d(dst, &map_w, it * 128, tile * 128, bar);
-                    gx_tma_2d(dst + A_BYTES, &map_x, it * 128, job * NT, bar);
+                    const uint32_t bar = full0 + s * 8, dst = ring0 + (uint32_t)s * slot;
+                    mbar_expect_tx(bar, slot);
+                    gx_tma_2d(dst, &map_w, (k_first + it) * 128, tile * 128, bar);
+                    gx_tma_2d(dst + GI_A_BYTES, &map_x, (k_first + it) * 128, job * NT, bar);
                 }
                 __syncwarp();
                 if (++s == S) { s = 0; ph ^= 1; }
@@ -95,7 +110,7 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
                 mbar_wait_spin(full0 + s * 8, ph, p.status, 19);
                 gx_fence_after();
                 if (elect_one()) {
-                    const uint64_t dA = d0 + (uint64_t)(((uint32_t)s * SLOT) >> 4), dB = dA + (A_BYTES >> 4);
+                    const uint64_t dA = d0 + (uint64_t)(((uint32_t)s * slot) >> 4), dB = dA + (GI_A_BYTES >> 4);
                     #pragma unroll
                     for (int kb = 0; kb < 4; ++kb)
                         asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -123,14 +138,16 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
                 float d[16];
                 gx_ld16(tq + (uint32_t)(buf * NT + c0), d);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (row < p.N) {
+                if (SPLIT) {                           // sums [token][128 rows], where the operands were
+                    int* o = reinterpret_cast<int*>(smem + pad) + c0 * 128 + q4 * 32 + lane;
+                    #pragma unroll
+                    for (int j = 0; j < 16; ++j) o[j * 128] = __float_as_int(d[j]);
+                } else if (row < p.N) {
                     const size_t o = (size_t)(m0 + c0) * p.N + row;
                     #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         if (c0 + j >= rows) break;
-                        const float v = __fmul_rn(__fmul_rn(__int2float_rn(__float_as_int(d[j])), sxs[buf][c0 + j]), sw);
-                        if (BF16) static_cast<__nv_bfloat16*>(p.y)[o + (size_t)j * p.N] = __float2bfloat16_rn(v);
-                        else static_cast<float*>(p.y)[o + (size_t)j * p.N] = v;
+                        gi_store(p.y, o + (size_t)j * p.N, __float_as_int(d[j]), sxs[buf][c0 + j], sw, BF16);
                     }
                 }
             }
@@ -140,32 +157,60 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
         }
     }
     gx_fence_before();
-    __syncthreads();
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(GI_TMEM_COLS));
+    __syncwarp();
+    if (SPLIT) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        const int tile = first / p.n_jobs, m0 = (first - tile * p.n_jobs) * NT, rows = min(NT, p.M - m0);
+        const int c1 = rows * (rank + 1) / p.split;
+        const int n = tile * 128 + (tid & 127);
+        const float sw = n < p.N ? p.sw[n] : 0.f;
+        const int* part = reinterpret_cast<const int*>(smem + pad) + (tid & 127);
+        for (int c = rows * rank / p.split + (tid >> 7); c < c1; c += GI_THREADS / 128) {
+            int v[GI_MAX_SPLIT];
+            #pragma unroll
+            for (int r = 0; r < GI_MAX_SPLIT; ++r) v[r] = r < p.split ? cluster.map_shared_rank(part, r)[c * 128] : 0;
+            int acc = 0;
+            #pragma unroll
+            for (int r = 0; r < GI_MAX_SPLIT; ++r) acc += v[r];
+            if (n < p.N) gi_store(p.y, (size_t)(m0 + c) * p.N + n, acc, sxs[0][c], sw, BF16);
+        }
+        cluster.sync();
+    } else __syncthreads();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(p.tmem_cols));
 }
 
-template <int NT, bool BF16>
-static int gi_launch(GiParams p, const b200_i8_rows* W, const b200_i8_rows* x, int K, cudaStream_t s) {
+template <bool BF16, bool SPLIT>
+static int gi_launch(GiParams& p, const b200_i8_rows* W, const b200_i8_rows* x, int K, cudaStream_t s) {
     CUtensorMap mw, mx;
     const size_t pitch = i8_pitch(K);
     if (!tmap_u8_pitched(&mw, W->q, (size_t)p.N, (size_t)K, pitch, 128, 128, true, true) ||
-        !tmap_u8_pitched(&mx, x->q, (size_t)p.M, (size_t)K, pitch, 128, NT, true, true)) return B200_ENOTIMPL;
-    auto kern = k_gemm_i8<NT, BF16>;
-    constexpr size_t slot = 16384 + NT * 128;
-    constexpr int most = (int)std::min<size_t>(GI_MAX_STAGES, (227 * 1024 - 1024 - 4096) / slot);      // 4 KB: static shared memory
-    constexpr size_t smem = most * slot + 1024;
+        !tmap_u8_pitched(&mx, x->q, (size_t)p.M, (size_t)K, pitch, 128, p.NT, true, true)) return B200_ENOTIMPL;
+    auto kern = k_gemm_i8<BF16, SPLIT>;
+    const size_t most = SPLIT ? GI_SMEM_SPLIT : GI_SMEM, slot = GI_A_BYTES + (size_t)p.NT * 128;
     static bool ready[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return launch_failed("gemm_i8: cudaGetDevice");
     if (dev < 0 || dev >= 64 || !ready[dev]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
             return launch_failed("gemm_i8: cudaFuncSetAttribute");
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    p.stages = most;
-    p.n_jobs = (p.M + NT - 1) / NT;
-    p.total = (p.N + 127) / 128 * p.n_jobs;
-    if (launch_pdl(kern, dim3(std::min(p.total, sm_count())), dim3(GI_THREADS), smem, s, p, mw, mx) != cudaSuccess) return launch_failed("k_gemm_i8");
+    p.stages = (int)std::min<size_t>(GI_MAX_STAGES, (most - 1024) / slot);
+    p.tmem_cols = 32;
+    while (p.tmem_cols < (SPLIT ? 1 : 2) * p.NT) p.tmem_cols *= 2;
+    // SPLIT: the sums of a tile lie where the operands were
+    const size_t smem = 1024 + std::max((size_t)p.stages * slot, SPLIT ? (size_t)p.NT * 512 : 0);
+    cudaLaunchConfig_t lc{};
+    lc.gridDim = dim3(SPLIT ? p.total * p.split : std::min(p.total, sm_count()));
+    lc.blockDim = dim3(GI_THREADS); lc.dynamicSmemBytes = smem; lc.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = p.split; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    lc.attrs = at; lc.numAttrs = SPLIT ? 2 : 1;
+    if (cudaLaunchKernelEx(&lc, kern, p, mw, mx) != cudaSuccess) return launch_failed("k_gemm_i8");
     return check_launch("k_gemm_i8");
 }
 
@@ -174,13 +219,16 @@ int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows*
     p.y = y; p.sw = W->scale; p.sx = x->scale; p.status = device_status_ptr();
     if (!p.status || !tmap_available()) return B200_ENOTIMPL;
     p.M = M; p.N = N; p.nst = (K + 127) / 128;
+    p.n_jobs = (M + GI_MAX_NT - 1) / GI_MAX_NT;
+    p.NT = ((M + p.n_jobs - 1) / p.n_jobs + 15) & ~15;        // the jobs' tokens evened out: 301 = 160 + 141
+    p.total = (N + 127) / 128 * p.n_jobs;
+    // CTAs per item: as many as one per SM leaves room for.  24 rows x [4096 x 12288], 32 items: 27.2 us with one, 18.0, 14.6 and
+    // 13.3 with 2, 3 and 4; but 16 rows x [12288 x 4096], 96 items: 12.4 with one, 14.0 with 2 on the SMs' second places.
+    p.split = std::max(1, std::min(std::min(sm_count() / p.total, GI_MAX_SPLIT), p.nst / 4));
+    if (p.NT > 128) p.split = 1;                       // the sums would not fit where the operands were
     credit(B200_CREDIT_GEMM, (double)N * K);
-    auto go = [&](auto bf) {
-        constexpr bool B = decltype(bf)::value;
-        return M <= 16 ? gi_launch<16, B>(p, W, x, K, s) : M <= 32 ? gi_launch<32, B>(p, W, x, K, s) : M <= 64 ? gi_launch<64, B>(p, W, x, K, s)
-             : M <= 128 ? gi_launch<128, B>(p, W, x, K, s) : gi_launch<256, B>(p, W, x, K, s);
-    };
-    return y_bf16 ? go(std::true_type{}) : go(std::false_type{});
+    if (p.split > 1) return y_bf16 ? gi_launch<true, true>(p, W, x, K, s) : gi_launch<false, true>(p, W, x, K, s);
+    return y_bf16 ? gi_launch<true, false>(p, W, x, K, s) : gi_launch<false, false>(p, W, x, K, s);
 }
 
 }  // namespace b200

@@ -89,6 +89,10 @@ int i8_quantize_launch(const void* x, int x_is_f32, size_t ldx, int rows, int K,
     return check_launch("k_i8_quantize");
 }
 
+// Up to so many bytes of activations the few-row kernel quantises them itself, in every CTA; beyond, in a launch of its own:
+// [4096 x 4096] 1 row 7.1 us and 7.9, 2 rows f32 (32 KB) 9.1 and 9.2, [12288 x 4096] 5 rows bf16 (40 KB) 18.9 and 15.0.
+constexpr size_t I8_GEMV_QUANT_BYTES = 32768;
+
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 }  // namespace b200
@@ -131,10 +135,13 @@ extern "C" int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const v
         if (int rc = check_x(x, x_dtype, ldx, M, K)) return rc;
         if (!ws) return B200_EINVAL;
         if ((uintptr_t)ws & 255) return B200_EALIGN;
+        if (gemv_i8_takes(M, K) && (size_t)M * K * (x_dtype == B200_F32 ? 4 : 2) <= I8_GEMV_QUANT_BYTES)
+            return gemv_i8(y, y_dtype == B200_BF16, W, x, x_dtype, ldx, nullptr, M, N, K, stream);
         int8_t* q = static_cast<int8_t*>(ws);
         float* scale = reinterpret_cast<float*>(q + up256((size_t)M * i8_pitch(K)));
         if (int rc = i8_quantize_launch(x, x_dtype == B200_F32, ldx, M, K, q, scale, stream)) return rc;
         xq = b200_i8_rows{q, scale};
     }
+    if (gemv_i8_takes(M, K)) return gemv_i8(y, y_dtype == B200_BF16, W, xq.q, B200_I8, 0, xq.scale, M, N, K, stream);
     return gemm_i8_wide(y, y_dtype == B200_BF16, W, &xq, M, N, K, stream);
 }

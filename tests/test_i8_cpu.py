@@ -65,3 +65,32 @@ def test_binding_refuses():
         P.I8Rows(torch.zeros(4, 16, dtype=torch.int8), torch.zeros(5), 8)
     with pytest.raises(P.B200Error):
         P.I8Rows.empty(0, 8, 'cpu')
+
+
+def test_binding_keeps_what_it_points_to(monkeypatch):
+    """The rows' descriptors are host structures: they have to be alive while the library reads them, temporaries too."""
+    import gc
+    import importlib
+    import weakref
+    import __graft_entry__ as G
+    P, b = pkg(), importlib.import_module(G.PKG_NAME + '.binding')
+    seen = []
+
+    class Fake:
+        def b200_i8_gemm(self, *a):
+            gc.collect()
+            seen.append([r() is not None for r in refs])
+            return 0
+
+    monkeypatch.setattr(b, '_device', lambda *t: None)
+    monkeypatch.setattr(b, '_stream', lambda s: None)
+    monkeypatch.setattr(b, 'lib', lambda: Fake())
+    refs = []
+
+    def rows():
+        r = P.I8Rows(torch.zeros((4, 16), dtype=torch.int8), torch.zeros(4), 16)
+        refs.append(weakref.ref(r))
+        return r
+
+    b.i8_gemm(rows(), rows())
+    assert seen == [[True, True]]
