@@ -180,6 +180,166 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
     if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(p.tmem_cols));
 }
 
+// ---- many tokens: two CTAs of a cluster share a tile of 256 weight rows x NT <= 256 tokens (cta_group::2) -------------------
+// One CTA's tile of 128 x 256 takes in 48 KB per step of 512 clocks of MMA, 94 bytes per clock: more than an SM's share of L2.  The pair's
+// CTAs bring 128 weight rows and half of the tokens each, 32 KB.  The first CTA issues the MMAs for both; both load into their own
+// shared memory and signal the first one's barrier; a commit frees the stage in both.  Plain loads, no multicast.
+__device__ __forceinline__ uint32_t gi_mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void gi_tma_pair(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void gi_commit_pair(uint32_t bar) {         // arrives on the barrier at this offset in both CTAs
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 :: "r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void gi_arrive_remote(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(GI_THREADS, 1) __cluster_dims__(2, 1, 1)
+k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ uint64_t full_bar[GI_MAX_STAGES], empty_bar[GI_MAX_STAGES], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_base_s;
+    __shared__ float sxs[2][GI_MAX_NT];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int S = p.stages, NT = p.NT, nst = p.nst, rank = (int)cluster.block_rank();
+    const uint32_t slot = GI_A_BYTES + (uint32_t)NT * 64u;
+    pdl_wait();                                        // before TMEM is taken, as above
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_base_s)), "r"(p.tmem_cols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    } else if (warp == 1) {
+        if (lane < S) { mbar_init(smem_u32(&full_bar[lane]), 1); mbar_init(smem_u32(&empty_bar[lane]), 1); }
+        if (lane < 2) { mbar_init(smem_u32(&acc_full[lane]), 1); mbar_init(smem_u32(&acc_empty[lane]), 16); }
+        mbar_fence_init();
+    }
+    gx_fence_before();
+    __syncwarp();
+    cluster.sync();                                    // both CTAs' barriers stand
+    gx_fence_after();
+    pdl_launch_dependents();
+    const uint32_t tmem = tmem_base_s;
+    const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+    const int n_items = (p.total - first + stride - 1) / stride;
+    const uint32_t ring0 = smem_u32(smem) + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
+    const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]);
+
+    if (warp == 0) {
+        const uint32_t lead0 = gi_mapa(full0, 0);
+        int s = 0; uint32_t ph = 1;
+        for (int i = 0; i < n_items; ++i) {
+            const int q = first + i * stride, tile = q / p.n_jobs, job = q - tile * p.n_jobs;
+            for (int it = 0; it < nst; ++it) {
+                mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
+                if (elect_one()) {
+                    const uint32_t bar = lead0 + s * 8, dst = ring0 + (uint32_t)s * slot;
+                    if (rank == 0) mbar_expect_tx(full0 + s * 8, 2 * slot);          // of both CTAs
+                    gi_tma_pair(dst, &map_w, it * 128, tile * 256 + rank * 128, bar);
+                    gi_tma_pair(dst + GI_A_BYTES, &map_x, it * 128, job * NT + rank * (NT / 2), bar);
+                }
+                __syncwarp();
+                if (++s == S) { s = 0; ph ^= 1; }
+            }
+        }
+        for (int k = 0; k < S; ++k) {                  // the last commits have arrived
+            mbar_wait_spin(empty0 + s * 8, ph, p.status, 17);
+            if (++s == S) { s = 0; ph ^= 1; }
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((256u >> 4) << 24);
+            const uint64_t d0 = gx_desc(ring0);
+            int s = 0; uint32_t ph = 0;
+            for (int i = 0; i < n_items; ++i) {
+                const int buf = i & 1, use = i >> 1;
+                if (use > 0) mbar_wait_spin(smem_u32(&acc_empty[buf]), (use - 1) & 1, p.status, 18);
+                const uint32_t tD = tmem + (uint32_t)(buf * NT);
+                for (int it = 0; it < nst; ++it) {
+                    mbar_wait_spin(full0 + s * 8, ph, p.status, 19);
+                    gx_fence_after();
+                    if (elect_one()) {
+                        const uint64_t dA = d0 + (uint64_t)(((uint32_t)s * slot) >> 4), dB = dA + (GI_A_BYTES >> 4);
+                        #pragma unroll
+                        for (int kb = 0; kb < 4; ++kb)
+                            asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                                         " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}"
+                                         :: "r"(tD), "l"(dA + kb * 2), "l"(dB + kb * 2), "r"(idesc), "r"((uint32_t)(it | kb)) : "memory");
+                        gi_commit_pair(empty0 + s * 8);
+                        if (it == nst - 1) gi_commit_pair(smem_u32(&acc_full[buf]));
+                    }
+                    __syncwarp();
+                    if (++s == S) { s = 0; ph ^= 1; }
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        const int te = tid - 128, grp = te >> 7, q4 = warp & 3;
+        const uint32_t tq = tmem + ((uint32_t)(q4 * 32) << 16);
+        const uint32_t done = gi_mapa(smem_u32(&acc_empty[0]), 0);
+        for (int i = 0; i < n_items; ++i) {
+            const int q = first + i * stride, tile = q / p.n_jobs, m0 = (q - tile * p.n_jobs) * NT, rows = min(NT, p.M - m0);
+            const int buf = i & 1, row = tile * 256 + rank * 128 + q4 * 32 + lane;
+            if (te < rows) sxs[buf][te] = p.sx[m0 + te];
+            const float sw = row < p.N ? p.sw[row] : 0.f;
+            named_sync(1, 256);
+            mbar_wait_spin(smem_u32(&acc_full[buf]), (i >> 1) & 1, p.status, 20);
+            gx_fence_after();
+            for (int c0 = grp * 16; c0 < rows; c0 += 32) {
+                float d[16];
+                gx_ld16(tq + (uint32_t)(buf * NT + c0), d);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (row < p.N) {
+                    const size_t o = (size_t)(m0 + c0) * p.N + row;
+                    #pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if (c0 + j >= rows) break;
+                        gi_store(p.y, o + (size_t)j * p.N, __float_as_int(d[j]), sxs[buf][c0 + j], sw, BF16);
+                    }
+                }
+            }
+            gx_fence_before();
+            __syncwarp();
+            if (lane == 0) gi_arrive_remote(done + buf * 8);
+        }
+    }
+    gx_fence_before();
+    __syncwarp();
+    cluster.sync();                                    // nothing of the other CTA's is under way to this one any more
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(p.tmem_cols));
+}
+
+template <bool BF16>
+static int gi_launch_pair(GiParams& p, const b200_i8_rows* W, const b200_i8_rows* x, int K, cudaStream_t s) {
+    CUtensorMap mw, mx;
+    const size_t pitch = i8_pitch(K);
+    if (!tmap_u8_pitched(&mw, W->q, (size_t)p.N, (size_t)K, pitch, 128, 128, true, true) ||
+        !tmap_u8_pitched(&mx, x->q, (size_t)p.M, (size_t)K, pitch, 128, p.NT / 2, true, true)) return B200_ENOTIMPL;
+    auto kern = k_gemm_i8_pair<BF16>;
+    const size_t slot = GI_A_BYTES + (size_t)p.NT * 64;
+    static bool ready[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return launch_failed("gemm_i8: cudaGetDevice");
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GI_SMEM) != cudaSuccess)
+            return launch_failed("gemm_i8: cudaFuncSetAttribute");
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    p.stages = (int)std::min<size_t>(GI_MAX_STAGES, (GI_SMEM - 1024) / slot);
+    p.tmem_cols = 32;
+    while (p.tmem_cols < 2 * p.NT) p.tmem_cols *= 2;
+    if (launch_pdl(kern, dim3(2 * std::min(p.total, sm_count() / 2)), dim3(GI_THREADS), 1024 + p.stages * slot, s, p, mw, mx) != cudaSuccess)
+        return launch_failed("k_gemm_i8_pair");
+    return check_launch("k_gemm_i8_pair");
+}
+
 template <bool BF16, bool SPLIT>
 static int gi_launch(GiParams& p, const b200_i8_rows* W, const b200_i8_rows* x, int K, cudaStream_t s) {
     CUtensorMap mw, mx;
@@ -227,6 +387,13 @@ int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows*
     p.split = std::max(1, std::min(std::min(sm_count() / p.total, GI_MAX_SPLIT), p.nst / 4));
     if (p.NT > 128) p.split = 1;                       // the sums would not fit where the operands were
     credit(B200_CREDIT_GEMM, (double)N * K);
+    // More than one tile of tokens: a pair of CTAs per tile.  [12288 x 4096] 2048 rows 80.6 us with single CTAs, 70.0 in pairs;
+    // 301 rows x [8192 x 4096] 15.4 and 14.3; 777 rows x [5003 x 2051] 24.4 and 21.0.
+    if (M > 128) {
+        p.NT = (p.NT + 31) & ~31;
+        p.total = (N + 255) / 256 * p.n_jobs;
+        return y_bf16 ? gi_launch_pair<true>(p, W, x, K, s) : gi_launch_pair<false>(p, W, x, K, s);
+    }
     if (p.split > 1) return y_bf16 ? gi_launch<true, true>(p, W, x, K, s) : gi_launch<false, true>(p, W, x, K, s);
     return y_bf16 ? gi_launch<true, false>(p, W, x, K, s) : gi_launch<false, false>(p, W, x, K, s);
 }
