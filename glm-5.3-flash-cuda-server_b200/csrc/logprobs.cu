@@ -2,21 +2,24 @@
 //
 //   m = max x      S = sum exp(x - m)      log p(t) = (x_t - m) - ln S      H = ln S - (1 / S) sum (x - m) exp(x - m)
 //
-// A cluster of CTAs takes a row, each CTA a contiguous part of it; parts are joined over distributed shared memory.
+// A cluster of CTAs takes a row, each CTA a contiguous part of it, which bulk copies bring through a ring in shared memory; parts
+// are joined over distributed shared memory.
 //
 // Statistics.  Every thread keeps (m, n, S, T): n elements equal to m (they count as exactly 1 and are not added), S and T in base 2
 // over the others:
 //   S = sum 2^d,  T = sum d 2^d,  d = (x - m) log2 e.
 // So S is what is left beside the likeliest token, and ln(1 + S) of a token that is nearly certain keeps its relative precision
-// (1 + S in f32 would not).  The threads start from the maximum of the CTA's first tile; a vector that holds nothing above it
-// (nearly all) takes the short path: one multiply-add, one exponential, two sums per element.  d is the multiply-add
-// fma(x, log2 e, -fl(m log2 e)): its distance from (x - m) log2 e is the same for every element and corrected when parts are joined.
+// (1 + S in f32 would not).  The threads start from the maximum of the CTA's first tile; a thread whose part of a tile holds nothing
+// above it (nearly all) takes the short path: one multiply-add, one exponential, two sums per element.  d is the multiply-add
+// fma(x, log2 e, -fl(m log2 e)): its distance from (x - m) log2 e is the same for every element and corrected when m changes.
 //
-// The likeliest tokens.  Order: logit descending, then index ascending, as one 64-bit key.  Every thread has the largest key of its
-// part of the first tile; the top-th largest of these is a bound that at least `top` elements reach, and later elements count only
-// above its value (an equal one has a larger index).  Those go to a list in shared memory, a few hundred for a vocabulary of 154880
-// in no particular order, from which warps sort 32 at a time and merge.  A list that overflows (logits in ascending order; a first
-// tile of masked tokens before many others) is dropped, and the CTA finds its bound by radix selection over its part instead.
+// The likeliest tokens.  Order: logit descending, then index ascending, as one 64-bit key.  A bound is a value that at least `top`
+// elements reach: the top-th of the two largest maxima of every warp.  The first tile gives one, and later elements count only
+// above it (an equal one has a larger index).  Vectors whose maximum counts go to a list in shared memory, and after tiles 1, 3,
+// 7, ... the list gives a higher bound: some 200 vectors of a vocabulary of 154880 in no particular order.  In the end the elements
+// of these vectors that reach the last bound, little more than `top`, are put in order by counting who is larger.  A list that
+// overflows (logits in ascending order; a first tile of masked tokens before many others; thousands of equal logits) is dropped,
+// and the CTA finds the top-th key by radix selection over its part instead.
 #include "b200_internal.h"
 #include "tma_pipe.cuh"
 #include <cuda_bf16.h>
@@ -27,72 +30,103 @@ namespace b200 {
 namespace cg = cooperative_groups;
 
 constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
-constexpr int LP_LIST = 2048;                      // candidates of a CTA
-constexpr int LP_VECS = 4;                         // 16-byte loads a thread has in a tile
+constexpr int LP_LIST = 512;                       // candidates of a CTA
+constexpr int LP_VECS = 4;                         // 16-byte vectors of a tile that a thread has
+constexpr int LP_TILE = LP_VECS * LP_THREADS;      // vectors of a tile
+constexpr int LP_STAGES = 3;
 constexpr float LP_LOG2E = 1.44269504088896341f, LP_LN2 = 0.693147180559945309f;
+constexpr uint32_t LP_TILE_BYTES = LP_TILE * 16;
+constexpr size_t LP_SMEM = LP_STAGES * LP_TILE_BYTES;                                // two CTAs per SM
+static_assert(LP_LIST <= LP_THREADS && 2 * LP_WARPS == 32 && B200_LOGPROBS_TOP_MAX <= 32, "a bound is one of two maxima of each warp");
 
 struct LpParams {
     const void* x; const int32_t* tokens; float* lp; float* entropy; int32_t* top_ids; float* top_lp;
-    size_t ld; int V, G, top;
+    unsigned int* status; size_t ld; int V, G, top;
 };
 
 struct LpStat { float m, n, s, t; };               // see above; n as a float (n <= 2^24 exact; beyond it its last bit does not matter)
 
-// 64-bit key of logit x at index i: orders by x descending, then i ascending; never 0.  -0 and +0 are the same logit.
-__device__ __forceinline__ unsigned long long lp_key(float x, int i) {
+// Bits of logit x that order like it, never 0 but for a NaN.  -0 and +0 are the same logit.
+__device__ __forceinline__ uint32_t lp_ordered(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);
-    return ((unsigned long long)(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) << 32) | (uint32_t)~i;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ int lp_index(unsigned long long key) { return (int)~(uint32_t)key; }
-__device__ __forceinline__ float lp_value(unsigned long long key) {
-    const uint32_t o = (uint32_t)(key >> 32);
-    return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
-}
+__device__ __forceinline__ float lp_unordered(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o); }
+// 64-bit key of logit x at index i: orders by x descending, then i ascending.
+__device__ __forceinline__ unsigned long long lp_key(float x, int i) { return ((unsigned long long)lp_ordered(x) << 32) | (0x7fffffffu - (uint32_t)i); }
+__device__ __forceinline__ int lp_index(unsigned long long key) { return (int)(0x7fffffffu - (uint32_t)key); }
+__device__ __forceinline__ float lp_value(unsigned long long key) { return lp_unordered((uint32_t)(key >> 32)); }
 __device__ __forceinline__ float lp_exp2(float d) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d)); return e; }
 __device__ __forceinline__ float lp_max(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
 // d = (x - m) log2 e in two steps, for any finite x and m.  -216 and below: 2^d is zero, d finite.
 __device__ __forceinline__ float lp_d(float x, float m) { return fmaxf((x - m) * LP_LOG2E, -216.f); }
 
-// Joins b into a.  Parts without elements have m = -inf, n = s = t = 0.  s = t = NaN marks a row that holds +inf or NaN.
-__device__ __forceinline__ LpStat lp_join(LpStat a, LpStat b) {
-    if (a.m < b.m) { const LpStat c = a; a = b; b = c; }
-    if (a.m == b.m) return LpStat{a.m, a.n + b.n, a.s + b.s, a.t + b.t};
-    const float d = lp_d(b.m, a.m), f = exp2f(d), all = b.n + b.s;         // b.m == -inf: f = 0
-    return LpStat{a.m, a.n, fmaf(f, all, a.s), a.t + f * (b.t + all * d)};
-}
-__device__ __forceinline__ LpStat lp_shfl(LpStat a, int o) {
-    return LpStat{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.n, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-                  __shfl_xor_sync(0xffffffffu, a.t, o)};
+// The warp's parts as one, in every lane.  Parts without elements have m = -inf, n = s = t = 0; s = NaN marks a row that holds +inf or NaN.
+__device__ __forceinline__ LpStat lp_join(LpStat a) {
+    const float m = lp_unordered(__reduce_max_sync(0xffffffffu, lp_ordered(a.m)));
+    if (a.m != m) {
+        const float d = lp_d(a.m, m), f = exp2f(d), all = a.n + a.s;
+        a.t = f * (a.t + all * d); a.s = f * all; a.n = 0.f;
+    }
+    #pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        a.n += __shfl_xor_sync(0xffffffffu, a.n, o);
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+    }
+    return LpStat{m, a.n, a.s, a.t};
 }
 
-// A warp's 32 keys (one per lane), descending.
-__device__ __forceinline__ unsigned long long lp_stage(unsigned long long k, int j, bool keep_max) {
-    const unsigned long long o = __shfl_xor_sync(0xffffffffu, k, j);
-    return (o > k) == keep_max ? o : k;
-}
-__device__ __forceinline__ unsigned long long lp_sort(unsigned long long k, int lane) {
-    #pragma unroll
-    for (int n = 2; n <= 32; n <<= 1)
-        #pragma unroll
-        for (int j = n >> 1; j; j >>= 1) k = lp_stage(k, j, ((lane & j) == 0) == ((lane & n) == 0));
-    return k;
-}
-// The 32 largest of two descending lists, descending.
-__device__ __forceinline__ unsigned long long lp_merge(unsigned long long a, unsigned long long b, int lane) {
-    const unsigned long long r = __shfl_sync(0xffffffffu, b, 31 - lane);
-    a = a > r ? a : r;
-    #pragma unroll
-    for (int j = 16; j; j >>= 1) a = lp_stage(a, j, (lane & j) == 0);
-    return a;
-}
-// lists[0] <- the 32 largest of lists[0 .. n - 1] (n a power of two); every thread calls it.
-__device__ __forceinline__ void lp_tree(unsigned long long (*lists)[32], int n, int warp, int lane) {
-    for (int h = n >> 1; h; h >>= 1) {
-        __syncthreads();
-        if (warp < h) lists[warp][lane] = lp_merge(lists[warp][lane], lists[warp + h][lane], lane);
-    }
+// A bound: the top-th of the two largest k of every warp, 0 if there are not so many.  Every thread calls it and gets it; w: 32 words.
+__device__ __noinline__ uint32_t lp_bound(uint32_t k, int top, uint32_t* w) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t first = __reduce_max_sync(0xffffffffu, k);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, k == first)) - 1) k = 0u;
+    const uint32_t second = __reduce_max_sync(0xffffffffu, k);
     __syncthreads();
+    if (lane == 0) { w[2 * warp] = first; w[2 * warp + 1] = second; }
+    __syncthreads();
+    const uint32_t v = w[lane];
+    int r = 0;
+    #pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const uint32_t o = __shfl_sync(0xffffffffu, v, i);
+        r += o > v || (o == v && i < lane);
+    }
+    return __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, r == top - 1)) - 1);
+}
+
+// best[0 .. top - 1] <- the largest of list[0 .. n - 1], descending; all keys differ.
+__device__ __noinline__ void lp_rank(const unsigned long long* list, int n, int top, unsigned long long* best) {
+    for (int c = threadIdx.x; c < n; c += LP_THREADS) {
+        const unsigned long long k = list[c];
+        int r = 0;
+        #pragma unroll 8
+        for (int i = 0; i < n; ++i) r += list[i] > k;
+        if (r < top) best[r] = k;
+    }
+}
+
+__device__ __forceinline__ unsigned long long lp_pack(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 lp_unpack2(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ unsigned long long lp_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long lp_add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 template <bool F32> struct LpVec { static constexpr int N = F32 ? 4 : 8; };
@@ -106,15 +140,32 @@ __device__ __forceinline__ void lp_unpack(const uint4& a, float (&v)[LpVec<F32>:
     }
 }
 
+// The larger of two words: an f32 each, or two bf16 each.  A NaN wins.
+template <bool F32>
+__device__ __forceinline__ uint32_t lp_maxw(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if (F32) r = __float_as_uint(lp_max(__uint_as_float(a), __uint_as_float(b)));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <bool F32>
+__device__ __forceinline__ float lp_maxof(uint32_t w) {
+    return F32 ? __uint_as_float(w) : lp_max(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
 template <bool F32>
 __global__ void __launch_bounds__(LP_THREADS, 2)
 k_token_logprobs(const __grid_constant__ LpParams p) {
     constexpr int NV = LpVec<F32>::N;
-    __shared__ unsigned long long list[LP_LIST];
-    __shared__ unsigned long long lists[LP_WARPS][32];
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ uint64_t full_bar[LP_STAGES], empty_bar[LP_STAGES];
+    __shared__ unsigned long long vecs[LP_LIST];       // candidates: (ordered maximum, vector)
+    __shared__ unsigned long long list[LP_LIST];       // keys
+    __shared__ unsigned long long best[B200_LOGPROBS_TOP_MAX];      // this CTA's, read by the cluster's first CTA
+    __shared__ uint32_t words[32];
     __shared__ LpStat stats[LP_WARPS];
     __shared__ LpStat part;                            // this CTA's, read by the cluster's first CTA
-    __shared__ int count;
+    __shared__ int n_vecs, n_list;
     __shared__ unsigned int hist[256];
     __shared__ unsigned int pick[2];
     cg::cluster_group cluster = cg::this_cluster();
@@ -122,6 +173,12 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const size_t row = blockIdx.x / C;
     const int V = p.V, top = p.top;
+    if (tid == 0) {
+        n_vecs = n_list = 0;
+        #pragma unroll
+        for (int i = 0; i < LP_STAGES; ++i) { mbar_init(smem_u32(&full_bar[i]), 1); mbar_init(smem_u32(&empty_bar[i]), LP_WARPS); }
+        mbar_fence_init();
+    }
     pdl_launch_dependents();
     pdl_wait();
 
@@ -138,47 +195,68 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     if (rank == 0 && tid < head) si = tid;
     if (rank == C - 1 && tid >= 32 && tid - 32 < V - head - nb * NV) si = head + nb * NV + tid - 32;
 
-    uint4 a[LP_VECS];
-    auto load = [&](int v) {
-        #pragma unroll
-        for (int u = 0; u < LP_VECS; ++u) {
-            const int i = v + u * LP_THREADS + tid;
-            if (i < v1) a[u] = __ldcs(xv + i);
-        }
+    const int nt = (v1 - v0 + LP_TILE - 1) / LP_TILE;
+    auto request = [&](int t) {                        // one thread: tile t into its stage
+        const uint32_t bytes = min(LP_TILE_BYTES, (uint32_t)(v1 - v0 - t * LP_TILE) * 16u), s = (uint32_t)t % LP_STAGES;
+        mbar_expect_tx(smem_u32(&full_bar[s]), bytes);
+        bulk_g2s(smem_u32(ring) + s * LP_TILE_BYTES, xv + v0 + t * LP_TILE, bytes, smem_u32(&full_bar[s]));
     };
-    if (tid == 0) count = 0;
-    load(v0);
+    if (tid == 0)
+        for (int t = 0; t < min(nt, LP_STAGES); ++t) request(t);
     const float sv = si >= 0 ? one(si) : -CUDART_INF_F;
+    __syncthreads();
 
-    // ---- first tile: the maximum, and the bound that `top` elements reach ----
-    float m = sv;
-    // (a tail element is no witness of the bound: elements between the tile and the tail come before it at the same value)
-    unsigned long long best = si >= 0 && si < head ? lp_key(sv, si) : 0ull;
+    constexpr uint32_t MASKED = F32 ? 0xff800000u : 0xff80ff80u;
+    uint4 a[LP_VECS];
+    auto load = [&](int t) {                           // vectors u * LP_THREADS + tid of tile t; -inf past the part
+        const int s = t % LP_STAGES;
+        if (warp == 0 && t > 0 && t + LP_STAGES - 1 < nt) {        // the stage of the tile before, once every warp has read it
+            mbar_wait_spin(smem_u32(&empty_bar[(t - 1) % LP_STAGES]), (uint32_t)((t - 1) / LP_STAGES) & 1u, p.status, 26);
+            if (elect_one()) request(t + LP_STAGES - 1);
+            __syncwarp();
+        }
+        mbar_wait_spin(smem_u32(&full_bar[s]), (uint32_t)(t / LP_STAGES) & 1u, p.status, 30);
+        const uint4* q = reinterpret_cast<const uint4*>(ring + (size_t)s * LP_TILE_BYTES) + tid;
+        const int left = v1 - v0 - t * LP_TILE;
+        if (left >= LP_TILE) {
+            #pragma unroll
+            for (int u = 0; u < LP_VECS; ++u) a[u] = q[u * LP_THREADS];
+        } else {
+            #pragma unroll
+            for (int u = 0; u < LP_VECS; ++u) a[u] = u * LP_THREADS + tid < left ? q[u * LP_THREADS] : make_uint4(MASKED, MASKED, MASKED, MASKED);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
+    };
+
+    // ---- first tile: the maximum, and a bound ----
+    if (nt) load(0);
+    else {
+        #pragma unroll
+        for (int u = 0; u < LP_VECS; ++u) a[u] = make_uint4(MASKED, MASKED, MASKED, MASKED);
+    }
+    float m = -CUDART_INF_F;
     #pragma unroll
     for (int u = 0; u < LP_VECS; ++u) {
-        const int i = v0 + u * LP_THREADS + tid;
-        if (i < v1) {
-            float v[NV];
-            lp_unpack<F32>(a[u], v);
-            #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                m = fmaxf(m, v[j]);
-                if (top) { const unsigned long long k = lp_key(v[j], head + i * NV + j); best = best > k ? best : k; }
-            }
-        }
+        float v[NV];
+        lp_unpack<F32>(a[u], v);
+        #pragma unroll
+        for (int j = 0; j < NV; ++j) m = fmaxf(m, v[j]);
     }
-    unsigned long long bound = ~0ull;
-    if (top) {
-        lists[warp][lane] = lp_sort(best, lane);
-        lp_tree(lists, LP_WARPS, warp, lane);
-        bound = lists[0][top - 1];
+    uint32_t lo = top ? lp_bound(v0 + tid < v1 ? lp_ordered(m) : 0u, top, words) : 0u;
+    {
+        const uint32_t most = __reduce_max_sync(0xffffffffu, lp_ordered(fmaxf(m, sv)));
+        if (lane == 0) hist[warp] = most;
+        __syncthreads();
+        m = lp_unordered(__reduce_max_sync(0xffffffffu, hist[lane & (LP_WARPS - 1)]));
     }
-    #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) stats[warp].m = m;
-    __syncthreads();
-    #pragma unroll
-    for (int w = 0; w < LP_WARPS; ++w) m = fmaxf(m, stats[w].m);
+    // A bound at a mask's value would make candidates of all masked elements.  Then what is above it counts, and if that is too little
+    // in the end, the first masked ones are added: `held` says whether `top` elements of earlier tiles reach the bound.
+    const float lowest = F32 ? -3.402823466e38f : -3.38953139e38f, low = lp_unordered(lo);
+    bool held = true;
+    if (lo && (low == lowest || low == -CUDART_INF_F)) { ++lo; held = false; }
+    // nothing to look for: +inf; no bound (fewer than 512 vectors): everything counts
+    float bv = !top ? CUDART_INF_F : lo ? lp_unordered(lo) : -CUDART_INF_F;
 
     // ---- the pass ----
     LpStat st{m, 0.f, 0.f, 0.f};
@@ -196,80 +274,132 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         drift = fine ? fmaf(-st.m, LP_LOG2E, m2) : 0.f;
         quick = fine ? st.m : -CUDART_INF_F;
     };
-    float qs = 0.f, qt = 0.f;                          // the short path's sums since the last change of st.m
+    unsigned long long qs = 0ull, qt = 0ull;           // the short path's sums since the last change of st.m, two halves
     auto flush = [&] {
-        const float f = exp2f(drift);
-        st.s = fmaf(f, qs, st.s);
-        st.t += f * fmaf(drift, qs, qt);
-        qs = qt = 0.f;
+        const float2 s2 = lp_unpack2(qs), t2 = lp_unpack2(qt);
+        const float s1 = s2.x + s2.y, t1 = t2.x + t2.y, f = exp2f(drift);
+        st.s = fmaf(f, s1, st.s);
+        st.t += f * fmaf(drift, s1, t1);
+        qs = qt = 0ull;
     };
     settle();
-    auto slow = [&](float v) {
-        if (!(v < CUDART_INF_F)) { st.s = st.t = CUDART_NAN_F; return; }
-        if (v == -CUDART_INF_F) return;
-        if (v > st.m) { flush(); raise(v); settle(); }
-        if (v == st.m) st.n += 1.f;
-        else { const float d = lp_d(v, st.m), e = exp2f(d); st.s += e; st.t = fmaf(e, d, st.t); }
+    auto quickly = [&](const uint4& w) {               // a vector whose elements are all below `quick`
+        float e[NV];
+        lp_unpack<F32>(w, e);
+        const unsigned long long l2 = lp_pack(LP_LOG2E, LP_LOG2E), n2 = lp_pack(-m2, -m2);
+        #pragma unroll
+        for (int j = 0; j < NV; j += 2) {
+            float2 d = lp_unpack2(lp_fma2(lp_pack(e[j], e[j + 1]), l2, n2));
+            d.x = fmaxf(d.x, -216.f); d.y = fmaxf(d.y, -216.f);
+            const unsigned long long f = lp_pack(lp_exp2(d.x), lp_exp2(d.y));
+            qs = lp_add2(qs, f); qt = lp_fma2(f, lp_pack(d.x, d.y), qt);
+        }
+    };
+    auto slow = [&](float v) {                         // an element that is no larger than st.m
+        const float d = lp_d(v, st.m), e = v == st.m ? 0.f : lp_exp2(d);
+        st.n += v == st.m ? 1.f : 0.f;
+        st.s += e; st.t = fmaf(e, d, st.t);
     };
     auto push = [&](float v, int i) {
-        const int c = atomicAdd(&count, 1);
+        const int c = atomicAdd(&n_list, 1);
         if (c < LP_LIST) list[c] = lp_key(v, i);
     };
-    if (si >= 0) { slow(sv); if (top) push(sv, si); }
-    const float bv = top ? lp_value(bound) : CUDART_INF_F;                // bound 0 (fewer elements than `top`): a NaN, and everything of the tile is pushed
-    for (int v = v0; v < v1; v += LP_VECS * LP_THREADS) {
-        uint4 b[LP_VECS];
+    #pragma unroll 1
+    for (int t = 0; t < nt; ++t) {
+        uint32_t c[LP_VECS];                           // the vectors' maxima, a NaN if they hold one (bf16: of even and of odd elements)
         #pragma unroll
-        for (int u = 0; u < LP_VECS; ++u) b[u] = a[u];
-        if (v + LP_VECS * LP_THREADS < v1) load(v + LP_VECS * LP_THREADS);
-        #pragma unroll
-        for (int u = 0; u < LP_VECS; ++u) {
-            const int i = v + u * LP_THREADS + tid;
-            if (i >= v1) continue;
-            float e[NV];
-            lp_unpack<F32>(b[u], e);
-            float c = e[0];
+        for (int u = 0; u < LP_VECS; ++u) c[u] = lp_maxw<F32>(lp_maxw<F32>(a[u].x, a[u].y), lp_maxw<F32>(a[u].z, a[u].w));
+        const float most = lp_maxof<F32>(lp_maxw<F32>(lp_maxw<F32>(c[0], c[1]), lp_maxw<F32>(c[2], c[3])));
+        if (most < quick) {
             #pragma unroll
-            for (int j = 1; j < NV; ++j) c = lp_max(c, e[j]);
-            if (c < quick) {
+            for (int u = 0; u < LP_VECS; ++u) quickly(a[u]);
+        } else if (!(most < CUDART_INF_F)) st.s = st.t = CUDART_NAN_F;
+        else if (most > -CUDART_INF_F) {               // a new maximum, or an equal one: those that equal it are counted, not added
+            if (most > st.m) { flush(); raise(most); settle(); }
+            #pragma unroll 1
+            for (int u = 0; u < LP_VECS; ++u) {
+                uint4 w = a[0];
                 #pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const float d = fmaxf(fmaf(e[j], LP_LOG2E, -m2), -216.f), f = lp_exp2(d);
-                    qs += f; qt = fmaf(f, d, qt);
-                }
-            } else {
-                #pragma unroll
-                for (int j = 0; j < NV; ++j) slow(e[j]);
-            }
-            if (top) {
-                if (v == v0) {
+                for (int i = 1; i < LP_VECS; ++i) if (u == i) w = a[i];
+                #pragma unroll 1
+                for (int j = 0; j < 4; ++j) {
                     #pragma unroll
-                    for (int j = 0; j < NV; ++j) if (lp_key(e[j], head + i * NV + j) >= bound) push(e[j], head + i * NV + j);
-                } else if (c > bv) {
-                    #pragma unroll
-                    for (int j = 0; j < NV; ++j) if (e[j] > bv) push(e[j], head + i * NV + j);
+                    for (int h = 0; h < NV / 4; ++h) slow(__uint_as_float(F32 ? w.x : h ? w.x & 0xffff0000u : w.x << 16));
+                    w.x = w.y; w.y = w.z; w.z = w.w;
                 }
             }
         }
+        if (top && most >= bv) {
+            const int left = v1 - v0 - t * LP_TILE;
+            #pragma unroll
+            for (int u = 0; u < LP_VECS; ++u) {
+                const int i = u * LP_THREADS + tid;
+                const float cu = lp_maxof<F32>(c[u]);
+                if ((t == 0 || !held ? cu >= bv : cu > bv) && i < left) {
+                    const int e = atomicAdd(&n_vecs, 1);
+                    if (e < LP_LIST) vecs[e] = ((unsigned long long)lp_ordered(cu) << 32) | (uint32_t)(v0 + t * LP_TILE + i);
+                }
+            }
+        }
+        if (t + 1 < nt) load(t + 1);
+        if (!((t + 1) & (t + 2)) && t + 2 < nt) {      // tiles 1, 3, 7, ... are done and more than one is left
+            // the CTA's maximum so far for all, at places that do not change from run to run
+            const uint32_t most_o = __reduce_max_sync(0xffffffffu, lp_ordered(st.m));
+            __syncthreads();
+            if (lane == 0) hist[warp] = most_o;
+            const int n = n_vecs;
+            __syncthreads();
+            const float mm = lp_unordered(__reduce_max_sync(0xffffffffu, hist[lane & (LP_WARPS - 1)]));
+            if (mm > st.m) { flush(); raise(mm); settle(); }
+            if (top && n <= LP_LIST) {
+                const int e = lane * LP_WARPS + warp;  // entry e belongs to warp e % LP_WARPS, so that every warp has some
+                const uint32_t b = lp_bound(e < n ? (uint32_t)(vecs[e] >> 32) : 0u, top, words);
+                if (b >= lo && b) { lo = b; bv = lp_unordered(b); held = true; }
+            }
+        }
     }
+    // single elements; those of the tail come after all others
     flush();
+    if (si >= 0) {
+        if (!(sv < CUDART_INF_F)) st.s = st.t = CUDART_NAN_F;
+        else if (sv > -CUDART_INF_F) slow(sv);         // st.m started no lower
+        if (top && lp_ordered(sv) >= lo) push(sv, si);
+    }
 
     // ---- join the CTA's parts ----
-    #pragma unroll
-    for (int o = 16; o; o >>= 1) st = lp_join(st, lp_shfl(st, o));
-    __syncthreads();
+    st = lp_join(st);
     if (lane == 0) stats[warp] = st;
     __syncthreads();
     if (warp == 0) {
-        st = lane < LP_WARPS ? stats[lane] : LpStat{-CUDART_INF_F, 0.f, 0.f, 0.f};
-        #pragma unroll
-        for (int o = LP_WARPS / 2; o; o >>= 1) st = lp_join(st, lp_shfl(st, o));
+        st = lp_join(lane < LP_WARPS ? stats[lane] : LpStat{-CUDART_INF_F, 0.f, 0.f, 0.f});
         if (lane == 0) part = st;
     }
     if (top) {
-        int n = count;
-        if (n > LP_LIST) {
-            // ---- radix selection: the digits of the bound from the top, until what reaches it fits the list ----
+        const int n = n_vecs;
+        if (n <= LP_LIST) {
+            const int e = lane * LP_WARPS + warp;
+            lo = max(lo, lp_bound(e < n ? (uint32_t)(vecs[e] >> 32) : 0u, top, words));
+            if (tid < n && (uint32_t)(vecs[tid] >> 32) >= lo) {
+                const int q = (int)(uint32_t)vecs[tid];
+                float f[NV];
+                lp_unpack<F32>(xv[q], f);
+                #pragma unroll
+                for (int j = 0; j < NV; ++j) if (lp_ordered(f[j]) >= lo) push(f[j], head + q * NV + j);
+            }
+        }
+        __syncthreads();
+        if (n <= LP_LIST && n_list < top) {            // masked ones: no more than top - 1 others are among the first of the part
+            __syncthreads();
+            const int i = (rank == 0 ? 0 : head + v0 * NV) + tid;
+            if (tid < 2 * B200_LOGPROBS_TOP_MAX && i < (rank == C - 1 ? V : head + v1 * NV)) {
+                const float f = one(i);
+                if (f == low) push(f, i);
+            }
+            __syncthreads();
+        }
+        if ((n > LP_LIST || n_list > LP_LIST || n_list < top) && !(part.s != part.s)) {
+            // ---- radix selection: the digits of the top-th key from the top, until few enough reach it ----
+            constexpr unsigned int FEW = 128;
             unsigned long long prefix = 0ull;
             int want = top, shift = 56;
             auto each = [&](auto f) {                   // f(key), 0 for none; whole warps
@@ -303,42 +433,41 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
                 prefix |= (unsigned long long)pick[0] << shift;
                 want -= (int)pick[1];
                 // top - want elements are above the prefix, hist[digit] share it
-                if (shift == 0 || (unsigned int)(top - want) + hist[pick[0]] <= (unsigned int)LP_LIST) break;
+                if (shift == 0 || (unsigned int)(top - want) + hist[pick[0]] <= FEW) break;
             }
             __syncthreads();
-            if (tid == 0) count = 0;
+            if (tid == 0) n_list = 0;
             __syncthreads();
-            each([&](unsigned long long k) { if (k && k >= prefix) { const int c = atomicAdd(&count, 1); if (c < LP_LIST) list[c] = k; } });
+            each([&](unsigned long long k) { if (k && k >= prefix) { const int c = atomicAdd(&n_list, 1); if (c < LP_LIST) list[c] = k; } });
             __syncthreads();
-            n = min(count, LP_LIST);
         }
-        unsigned long long k = 0ull;
-        for (int c = warp * 32; c < n; c += LP_THREADS) {
-            const unsigned long long q = lp_sort(c + lane < n ? list[c + lane] : 0ull, lane);
-            k = lp_merge(k, q, lane);
-        }
-        lists[warp][lane] = k;
-        lp_tree(lists, LP_WARPS, warp, lane);
+        lp_rank(list, min(n_list, LP_LIST), top, best);
     }
 
     // ---- join the cluster's parts in its first CTA ----
-    LpStat all;
     if (C > 1) {
         cluster.sync();
         if (rank == 0) {
-            all = part;
-            for (int r = 1; r < C; ++r) all = lp_join(all, *cluster.map_shared_rank(&part, r));
+            LpStat all{-CUDART_INF_F, 0.f, 0.f, 0.f};
+            if (warp == 0 && lane < C) all = *cluster.map_shared_rank(&part, lane);
             if (top) {
-                if (warp > 0 && warp < C) lists[warp][lane] = (*cluster.map_shared_rank(&lists, warp))[0][lane];
-                lp_tree(lists, C, warp, lane);
+                // no CTA's last one is above the row's top-th
+                unsigned long long least = lane < C ? cluster.map_shared_rank(best, lane)[top - 1] : 0ull;
+                #pragma unroll
+                for (int o = 16; o; o >>= 1) { const unsigned long long q = __shfl_xor_sync(0xffffffffu, least, o); least = q > least ? q : least; }
+                if (tid == 0) n_list = 0;
+                __syncthreads();
+                const unsigned long long k = warp < C && lane < top ? cluster.map_shared_rank(best, warp)[lane] : 0ull;
+                if (k && k >= least) list[atomicAdd(&n_list, 1)] = k;
+                __syncthreads();
+                lp_rank(list, n_list, top, best);
             }
+            if (warp == 0) { all = lp_join(all); if (lane == 0) part = all; }
         }
         cluster.sync();
         if (rank) return;
-    } else {
-        __syncthreads();
-        all = part;
-    }
+    } else __syncthreads();
+    const LpStat all = part;
 
     // ---- results ----
     const bool bad = !(all.s <= CUDART_INF_F), none = !bad && all.n == 0.f;        // +inf or NaN in the row; every logit -inf
@@ -350,7 +479,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         p.lp[row * p.G + g] = t < 0 ? 0.f : t >= V ? CUDART_NAN_F : logp(one(t));
     }
     if (tid < top) {
-        const unsigned long long k = lists[0][tid];
+        const unsigned long long k = best[tid];
         p.top_ids[row * top + tid] = bad ? -1 : lp_index(k);
         p.top_lp[row * top + tid] = logp(lp_value(k));
     }
@@ -360,16 +489,25 @@ template <bool F32>
 static int lp_launch(const LpParams& p, int M, cudaStream_t s) {
     // CTAs per row: as many as leave the whole batch on the GPU at once (two CTAs per SM), and a tile's worth of work to each.
     int C = 8;
-    while (C > 1 && ((long long)M * C > 2 * sm_count() || p.V / C < LP_THREADS * LpVec<F32>::N)) C >>= 1;
+    while (C > 1 && ((long long)M * C > 2 * sm_count() || p.V / C < LP_TILE * LpVec<F32>::N)) C >>= 1;
+    auto kern = k_token_logprobs<F32>;
+    static bool ready[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return launch_failed("token_logprobs: cudaGetDevice");
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LP_SMEM) != cudaSuccess)
+            return launch_failed("token_logprobs: cudaFuncSetAttribute");
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
     cudaLaunchConfig_t lc{};
-    lc.gridDim = dim3((unsigned)M * C); lc.blockDim = dim3(LP_THREADS); lc.stream = s;
+    lc.gridDim = dim3((unsigned)M * C); lc.blockDim = dim3(LP_THREADS); lc.dynamicSmemBytes = LP_SMEM; lc.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = C; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
-    lc.attrs = at; lc.numAttrs = 2;
-    if (cudaLaunchKernelEx(&lc, k_token_logprobs<F32>, p) != cudaSuccess) return launch_failed("k_token_logprobs");
+    lc.attrs = at; lc.numAttrs = C > 1 ? 2 : 1;
+    if (cudaLaunchKernelEx(&lc, kern, p) != cudaSuccess) return launch_failed("k_token_logprobs");
     return check_launch("k_token_logprobs");
 }
 
@@ -384,6 +522,7 @@ extern "C" int b200_token_logprobs(const void* logits, int dtype, size_t ld, int
     if (top > B200_LOGPROBS_TOP_MAX || M > I8_MAX_ROWS || V > (1 << 30)) return B200_ELIMIT;
     if (((uintptr_t)logits & (dtype == B200_F32 ? 3 : 1)) || ((uintptr_t)tokens & 3) || ((uintptr_t)logprobs & 3) || ((uintptr_t)entropy & 3) ||
         ((uintptr_t)top_ids & 3) || ((uintptr_t)top_logprobs & 3)) return B200_EALIGN;
-    const LpParams p{logits, tokens, logprobs, entropy, top_ids, top_logprobs, ld, V, G, top};
+    LpParams p{logits, tokens, logprobs, entropy, top_ids, top_logprobs, device_status_ptr(), ld, V, G, top};
+    if (!p.status) return B200_ENOTIMPL;
     return dtype == B200_F32 ? lp_launch<true>(p, M, stream) : lp_launch<false>(p, M, stream);
 }

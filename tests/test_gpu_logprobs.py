@@ -60,7 +60,8 @@ def check(x, tokens, top, out=None):
     eps = 2.0 ** -24
     r = (x.shape[1] / 512 + 164) * eps
     scale = np.nan_to_num(np.abs(ln_s), nan=0.0, posinf=0.0)[:, None]
-    tol = lambda w: r * (1 - np.exp(-scale)) + 4 * eps * (2 * np.where(np.isfinite(w), np.abs(w), 0) + 2 * scale) + 1e-38
+    # S / (1 + S) = 1 - exp(-ln(1 + S)), which double precision loses for S < 2^-53 unless it is taken as -expm1: r S is due there
+    tol = lambda w: r * -np.expm1(-scale) + 4 * eps * (2 * np.where(np.isfinite(w), np.abs(w), 0) + 2 * scale) + 1e-38
     close(lp, wlp, tol(wlp))
     close(tlp, wtlp, tol(wtlp))
     close(h, wh, 2 * r * np.where(np.isfinite(wh), wh, 0) + 4 * eps * np.where(np.isfinite(wh), wh, 0) + 1e-38)
