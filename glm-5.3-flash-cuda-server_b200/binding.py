@@ -339,13 +339,9 @@ def _want(ok, what):
 
 def _device(*tensors):
     """Kernels run on the current device's stream: every tensor has to lie there."""
-    for t in tensors:
-        if not t.is_cuda:
-            raise B200Error('tensors have to be on the current CUDA device')
-    dev = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t.get_device() != dev:
-            raise B200Error('tensors have to be on the current CUDA device')
+    devs = [t.get_device() for t in tensors]            # -1: not on a GPU
+    if min(devs) < 0 or devs.count(torch._C._cuda_getDevice()) != len(devs):
+        raise B200Error('tensors have to be on the current CUDA device')
 
 
 def _strided_rows(x, what):
@@ -435,34 +431,48 @@ def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
 LOGPROBS_TOP_MAX = 32
 
 
+class LogprobsOut(tuple):
+    """(logprobs [M, G], entropy [M], top_ids [M, top], top_logprobs [M, top]), checked once: token_logprobs_out."""
+
+    @classmethod
+    def of(cls, tensors, M, G, top):
+        lp, ent, ids, tlp = tensors
+        if (lp.shape != (M, G) or ent.shape != (M,) or ids.shape != (M, top) or tlp.shape != (M, top) or ids.dtype != torch.int32 or
+                not (lp.dtype == ent.dtype == tlp.dtype == torch.float32) or
+                not (lp.is_contiguous() and ent.is_contiguous() and ids.is_contiguous() and tlp.is_contiguous())):
+            raise B200Error('out has to be token_logprobs_out(tokens, top)')
+        self = cls(tensors)
+        self.size = (M, G, top)
+        return self
+
+
 def token_logprobs_out(tokens, top):
     """Output buffers of token_logprobs for these tokens."""
-    M, dev = tokens.shape[0], tokens.device
-    return (torch.empty(tokens.shape, dtype=torch.float32, device=dev), torch.empty(M, dtype=torch.float32, device=dev),
-            torch.empty((M, top), dtype=torch.int32, device=dev), torch.empty((M, top), dtype=torch.float32, device=dev))
+    _want(tokens.dim() == 2 and top >= 0, 'tokens has to be [M, G], top not negative')
+    M, G = tokens.shape
+    f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=tokens.device)
+    return LogprobsOut.of((f32(M, G), f32(M), torch.empty((M, top), dtype=torch.int32, device=tokens.device), f32(M, top)), M, G, top)
 
 
 def token_logprobs(logits, tokens, top=0, out=None, stream=None):
     """ln p of the given tokens (tokens int32 [M, G]; negative: none, 0), the entropy in nats, and the `top` likeliest tokens of every
     row of logits [M, V] (f32 or bf16): (logprobs [M, G], entropy [M], top_ids [M, top], top_logprobs [M, top])."""
     dt, M, V, ld = _strided_rows(logits, 'logits')
-    if tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != M or not tokens.is_contiguous():
+    shape = tokens.shape
+    if tokens.dtype != torch.int32 or len(shape) != 2 or shape[0] != M or not tokens.is_contiguous():
         raise B200Error('tokens has to be contiguous int32 [M, G]')
-    G = tokens.shape[1]
+    G = shape[1]
     if out is None:
-        _want(top >= 0, 'top may not be negative')
         out = token_logprobs_out(tokens, top)
+    elif type(out) is not LogprobsOut or out.size != (M, G, top):
+        out = LogprobsOut.of(out, M, G, top)
     lp, ent, ids, tlp = out
-    if (lp.shape != (M, G) or ent.shape != (M,) or ids.shape != (M, top) or tlp.shape != (M, top) or ids.dtype != torch.int32 or
-            not (lp.dtype == ent.dtype == tlp.dtype == torch.float32) or
-            not (lp.is_contiguous() and ent.is_contiguous() and ids.is_contiguous() and tlp.is_contiguous())):
-        raise B200Error('out has to be token_logprobs_out(tokens, top)')
     _device(logits, tokens, lp, ent, ids, tlp)
     rc = lib().b200_token_logprobs(logits.data_ptr(), dt, ld, M, V, tokens.data_ptr(), G, lp.data_ptr(), ent.data_ptr(), top, ids.data_ptr(),
                                    tlp.data_ptr(), _stream(stream))
     if rc:
         check(rc, 'b200_token_logprobs')
-    return lp, ent, ids, tlp
+    return out
 
 
 class MoeLayer:

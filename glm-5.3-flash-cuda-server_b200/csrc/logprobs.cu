@@ -29,15 +29,11 @@
 namespace b200 {
 namespace cg = cooperative_groups;
 
-constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_LIST = 512;                       // candidates of a CTA
 constexpr int LP_VECS = 4;                         // 16-byte vectors of a tile that a thread has
-constexpr int LP_TILE = LP_VECS * LP_THREADS;      // vectors of a tile
 constexpr int LP_STAGES = 3;
 constexpr float LP_LOG2E = 1.44269504088896341f, LP_LN2 = 0.693147180559945309f;
-constexpr uint32_t LP_TILE_BYTES = LP_TILE * 16;
-constexpr size_t LP_SMEM = LP_STAGES * LP_TILE_BYTES;                                // two CTAs per SM
-static_assert(LP_LIST <= LP_THREADS && 2 * LP_WARPS == 32 && B200_LOGPROBS_TOP_MAX <= 32, "a bound is one of two maxima of each warp");
+static_assert(B200_LOGPROBS_TOP_MAX <= 32, "a bound is one of 32 maxima");
 
 struct LpParams {
     const void* x; const int32_t* tokens; float* lp; float* entropy; int32_t* top_ids; float* top_lp;
@@ -78,26 +74,41 @@ __device__ __forceinline__ LpStat lp_join(LpStat a) {
     return LpStat{m, a.n, a.s, a.t};
 }
 
-// A bound: the top-th of the two largest k of every warp, 0 if there are not so many.  Every thread calls it and gets it; w: 32 words.
+// A bound: the top-th of the largest two (four) k of every one of 16 (8) warps, 0 if there are not so many.  Every thread calls it and gets
+// it; w: 32 words.
+template <int LP_THREADS>
 __device__ __noinline__ uint32_t lp_bound(uint32_t k, int top, uint32_t* w) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t first = __reduce_max_sync(0xffffffffu, k);
-    if (lane == __ffs(__ballot_sync(0xffffffffu, k == first)) - 1) k = 0u;
-    const uint32_t second = __reduce_max_sync(0xffffffffu, k);
-    __syncthreads();
-    if (lane == 0) { w[2 * warp] = first; w[2 * warp + 1] = second; }
-    __syncthreads();
-    const uint32_t v = w[lane];
-    int r = 0;
+    constexpr int EACH = 32 / (LP_THREADS / 32);
+    uint32_t most[EACH];
     #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const uint32_t o = __shfl_sync(0xffffffffu, v, i);
-        r += o > v || (o == v && i < lane);
+    for (int i = 0; i < EACH; ++i) {
+        most[i] = __reduce_max_sync(0xffffffffu, k);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, k == most[i])) - 1) k = 0u;
     }
-    return __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, r == top - 1)) - 1);
+    __syncthreads();
+    if (lane == 0) {
+        #pragma unroll
+        for (int i = 0; i < EACH; ++i) w[EACH * warp + i] = most[i];
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const uint32_t v = w[lane];
+        int r = 0;
+        #pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t o = __shfl_sync(0xffffffffu, v, i);
+            r += o > v || (o == v && i < lane);
+        }
+        __syncwarp();
+        if (r == top - 1) w[0] = v;
+    }
+    __syncthreads();
+    return w[0];
 }
 
 // best[0 .. top - 1] <- the largest of list[0 .. n - 1], descending; all keys differ.
+template <int LP_THREADS>
 __device__ __noinline__ void lp_rank(const unsigned long long* list, int n, int top, unsigned long long* best) {
     for (int c = threadIdx.x; c < n; c += LP_THREADS) {
         const unsigned long long k = list[c];
@@ -153,10 +164,12 @@ __device__ __forceinline__ float lp_maxof(uint32_t w) {
     return F32 ? __uint_as_float(w) : lp_max(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-template <bool F32>
-__global__ void __launch_bounds__(LP_THREADS, 2)
+template <bool F32, int LP_THREADS>
+__global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS)
 k_token_logprobs(const __grid_constant__ LpParams p) {
-    constexpr int NV = LpVec<F32>::N;
+    constexpr int NV = LpVec<F32>::N, LP_WARPS = LP_THREADS / 32;
+    constexpr int LP_TILE = LP_VECS * LP_THREADS;      // vectors
+    constexpr uint32_t LP_TILE_BYTES = LP_TILE * 16;
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ uint64_t full_bar[LP_STAGES], empty_bar[LP_STAGES];
     __shared__ unsigned long long vecs[LP_LIST];       // candidates: (ordered maximum, vector)
@@ -204,6 +217,13 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     if (tid == 0)
         for (int t = 0; t < min(nt, LP_STAGES); ++t) request(t);
     const float sv = si >= 0 ? one(si) : -CUDART_INF_F;
+    // this thread's given token, long before its log probability is known
+    int token = -1;
+    float token_x = 0.f;
+    if (rank == 0 && tid < p.G) {
+        token = p.tokens[row * p.G + tid];
+        if ((unsigned)token < (unsigned)V) token_x = one(token);
+    }
     __syncthreads();
 
     constexpr uint32_t MASKED = F32 ? 0xff800000u : 0xff80ff80u;
@@ -211,11 +231,11 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     auto load = [&](int t) {                           // vectors u * LP_THREADS + tid of tile t; -inf past the part
         const int s = t % LP_STAGES;
         if (warp == 0 && t > 0 && t + LP_STAGES - 1 < nt) {        // the stage of the tile before, once every warp has read it
-            mbar_wait_spin(smem_u32(&empty_bar[(t - 1) % LP_STAGES]), (uint32_t)((t - 1) / LP_STAGES) & 1u, p.status, 26);
+            mbar_wait(smem_u32(&empty_bar[(t - 1) % LP_STAGES]), (uint32_t)((t - 1) / LP_STAGES) & 1u, p.status, 26);
             if (elect_one()) request(t + LP_STAGES - 1);
             __syncwarp();
         }
-        mbar_wait_spin(smem_u32(&full_bar[s]), (uint32_t)(t / LP_STAGES) & 1u, p.status, 30);
+        mbar_wait(smem_u32(&full_bar[s]), (uint32_t)(t / LP_STAGES) & 1u, p.status, 30);
         const uint4* q = reinterpret_cast<const uint4*>(ring + (size_t)s * LP_TILE_BYTES) + tid;
         const int left = v1 - v0 - t * LP_TILE;
         if (left >= LP_TILE) {
@@ -243,7 +263,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         #pragma unroll
         for (int j = 0; j < NV; ++j) m = fmaxf(m, v[j]);
     }
-    uint32_t lo = top ? lp_bound(v0 + tid < v1 ? lp_ordered(m) : 0u, top, words) : 0u;
+    uint32_t lo = top ? lp_bound<LP_THREADS>(v0 + tid < v1 ? lp_ordered(m) : 0u, top, words) : 0u;
     {
         const uint32_t most = __reduce_max_sync(0xffffffffu, lp_ordered(fmaxf(m, sv)));
         if (lane == 0) hist[warp] = most;
@@ -304,6 +324,12 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         const int c = atomicAdd(&n_list, 1);
         if (c < LP_LIST) list[c] = lp_key(v, i);
     };
+    // the candidates' maxima, a thread's largest; entry e belongs to warp e % LP_WARPS, so that every warp has some
+    auto entry = [&](int n) {
+        uint32_t k = 0u;
+        for (int e = lane * LP_WARPS + warp; e < n; e += LP_THREADS) k = max(k, (uint32_t)(vecs[e] >> 32));
+        return k;
+    };
     #pragma unroll 1
     for (int t = 0; t < nt; ++t) {
         uint32_t c[LP_VECS];                           // the vectors' maxima, a NaN if they hold one (bf16: of even and of odd elements)
@@ -352,8 +378,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
             const float mm = lp_unordered(__reduce_max_sync(0xffffffffu, hist[lane & (LP_WARPS - 1)]));
             if (mm > st.m) { flush(); raise(mm); settle(); }
             if (top && n <= LP_LIST) {
-                const int e = lane * LP_WARPS + warp;  // entry e belongs to warp e % LP_WARPS, so that every warp has some
-                const uint32_t b = lp_bound(e < n ? (uint32_t)(vecs[e] >> 32) : 0u, top, words);
+                const uint32_t b = lp_bound<LP_THREADS>(entry(n), top, words);
                 if (b >= lo && b) { lo = b; bv = lp_unordered(b); held = true; }
             }
         }
@@ -377,12 +402,13 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     if (top) {
         const int n = n_vecs;
         if (n <= LP_LIST) {
-            const int e = lane * LP_WARPS + warp;
-            lo = max(lo, lp_bound(e < n ? (uint32_t)(vecs[e] >> 32) : 0u, top, words));
-            if (tid < n && (uint32_t)(vecs[tid] >> 32) >= lo) {
-                const int q = (int)(uint32_t)vecs[tid];
+            lo = max(lo, lp_bound<LP_THREADS>(entry(n), top, words));
+            for (int i = tid; i < n; i += LP_THREADS) {
+                if ((uint32_t)(vecs[i] >> 32) < lo) continue;
+                const int q = (int)(uint32_t)vecs[i];
                 float f[NV];
-                lp_unpack<F32>(xv[q], f);
+                const int o = q - v0, t = o / LP_TILE;             // the last tiles still lie in the ring
+                lp_unpack<F32>(t + LP_STAGES >= nt ? reinterpret_cast<const uint4*>(ring + (size_t)(t % LP_STAGES) * LP_TILE_BYTES)[o - t * LP_TILE] : xv[q], f);
                 #pragma unroll
                 for (int j = 0; j < NV; ++j) if (lp_ordered(f[j]) >= lo) push(f[j], head + q * NV + j);
             }
@@ -414,7 +440,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
             };
             for (;; shift -= 8) {
                 __syncthreads();
-                if (tid < 256) hist[tid] = 0u;
+                for (int i = tid; i < 256; i += LP_THREADS) hist[i] = 0u;
                 __syncthreads();
                 each([&](unsigned long long k) {
                     const bool in = k && (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
@@ -441,7 +467,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
             each([&](unsigned long long k) { if (k && k >= prefix) { const int c = atomicAdd(&n_list, 1); if (c < LP_LIST) list[c] = k; } });
             __syncthreads();
         }
-        lp_rank(list, min(n_list, LP_LIST), top, best);
+        lp_rank<LP_THREADS>(list, min(n_list, LP_LIST), top, best);
     }
 
     // ---- join the cluster's parts in its first CTA ----
@@ -457,17 +483,21 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
                 for (int o = 16; o; o >>= 1) { const unsigned long long q = __shfl_xor_sync(0xffffffffu, least, o); least = q > least ? q : least; }
                 if (tid == 0) n_list = 0;
                 __syncthreads();
-                const unsigned long long k = warp < C && lane < top ? cluster.map_shared_rank(best, warp)[lane] : 0ull;
-                if (k && k >= least) list[atomicAdd(&n_list, 1)] = k;
+                for (int r = warp; r < C; r += LP_WARPS) {
+                    const unsigned long long k = lane < top ? cluster.map_shared_rank(best, r)[lane] : 0ull;
+                    if (k && k >= least) list[atomicAdd(&n_list, 1)] = k;
+                }
                 __syncthreads();
-                lp_rank(list, n_list, top, best);
+                lp_rank<LP_THREADS>(list, n_list, top, best);
             }
-            if (warp == 0) { all = lp_join(all); if (lane == 0) part = all; }
+            if (warp == 0) { all = lp_join(all); if (lane == 0) stats[0] = all; }
         }
-        cluster.sync();
-        if (rank) return;
-    } else __syncthreads();
-    const LpStat all = part;
+        __syncwarp();
+        cluster.barrier_arrive();                      // the other CTAs' shared memory has been read
+        if (rank) { cluster.barrier_wait(); return; }
+    } else if (tid == 0) stats[0] = part;
+    __syncthreads();
+    const LpStat all = stats[0];
 
     // ---- results ----
     const bool bad = !(all.s <= CUDART_INF_F), none = !bad && all.n == 0.f;        // +inf or NaN in the row; every logit -inf
@@ -475,32 +505,34 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     auto logp = [&](float v) { return bad ? CUDART_NAN_F : none ? -CUDART_INF_F : (v - all.m) - ln_s; };
     if (tid == 0) p.entropy[row] = bad ? CUDART_NAN_F : none ? 0.f : fmaxf(ln_s - all.t * LP_LN2 / (all.n + all.s), 0.f);
     for (int g = tid; g < p.G; g += LP_THREADS) {
-        const int t = p.tokens[row * p.G + g];
-        p.lp[row * p.G + g] = t < 0 ? 0.f : t >= V ? CUDART_NAN_F : logp(one(t));
+        if (g >= LP_THREADS) {
+            token = p.tokens[row * p.G + g];
+            if ((unsigned)token < (unsigned)V) token_x = one(token);
+        }
+        p.lp[row * p.G + g] = token < 0 ? 0.f : token >= V ? CUDART_NAN_F : logp(token_x);
     }
     if (tid < top) {
         const unsigned long long k = best[tid];
         p.top_ids[row * top + tid] = bad ? -1 : lp_index(k);
         p.top_lp[row * top + tid] = logp(lp_value(k));
     }
+    if (C > 1) { __syncwarp(); cluster.barrier_wait(); }
 }
 
-template <bool F32>
-static int lp_launch(const LpParams& p, int M, cudaStream_t s) {
-    // CTAs per row: as many as leave the whole batch on the GPU at once (two CTAs per SM), and a tile's worth of work to each.
-    int C = 8;
-    while (C > 1 && ((long long)M * C > 2 * sm_count() || p.V / C < LP_TILE * LpVec<F32>::N)) C >>= 1;
-    auto kern = k_token_logprobs<F32>;
+template <bool F32, int THREADS>
+static int lp_launch(const LpParams& p, int M, int C, cudaStream_t s) {
+    auto kern = k_token_logprobs<F32, THREADS>;
+    constexpr size_t smem = (size_t)LP_STAGES * LP_VECS * THREADS * 16;
     static bool ready[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return launch_failed("token_logprobs: cudaGetDevice");
     if (dev < 0 || dev >= 64 || !ready[dev]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LP_SMEM) != cudaSuccess)
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
             return launch_failed("token_logprobs: cudaFuncSetAttribute");
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
     cudaLaunchConfig_t lc{};
-    lc.gridDim = dim3((unsigned)M * C); lc.blockDim = dim3(LP_THREADS); lc.dynamicSmemBytes = LP_SMEM; lc.stream = s;
+    lc.gridDim = dim3((unsigned)M * C); lc.blockDim = dim3(THREADS); lc.dynamicSmemBytes = smem; lc.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -509,6 +541,20 @@ static int lp_launch(const LpParams& p, int M, cudaStream_t s) {
     lc.attrs = at; lc.numAttrs = C > 1 ? 2 : 1;
     if (cudaLaunchKernelEx(&lc, kern, p) != cudaSuccess) return launch_failed("k_token_logprobs");
     return check_launch("k_token_logprobs");
+}
+
+template <bool F32>
+static int lp_choose(const LpParams& p, int M, cudaStream_t s) {
+    // CTAs per row: as many as leave the whole batch on the GPU at once (two CTAs per SM), and a tile's worth of work to each.
+    int C = 8;
+    while (C > 1 && ((long long)M * C > 2 * sm_count() || p.V / C < 512 * LP_VECS * LpVec<F32>::N)) C >>= 1;
+    // Threads per CTA (1024 per SM in any case): few large CTAs where a row's time counts, small ones, whose barriers cost the others
+    // nothing, where there are rows enough.  us with 512 / 256 / 128: [1 x 154880] f32, top 5 10.8 / 12.8 / 17.6; [200 x 20000] f32,
+    // top 20 14.4 / 16.4 / 23.3; [300 x 1000] f32, top 5 12.1 / 6.9 / 7.4; [2048 x 154880] f32, top 20 227 / 222 / 234, bf16
+    // 194 / 177 / 172; [2000 x 20000] bf16, top 20 71 / 62 / 56; [2000 x 600] bf16, top 5 54 / 34 / 22.
+    const size_t vecs = (size_t)p.V / LpVec<F32>::N;
+    if (M > 4 * sm_count()) return vecs <= 8192 ? lp_launch<F32, 128>(p, M, C, s) : lp_launch<F32, 256>(p, M, C, s);
+    return C == 1 && vecs <= 1024 ? lp_launch<F32, 256>(p, M, C, s) : lp_launch<F32, 512>(p, M, C, s);
 }
 
 }  // namespace b200
@@ -524,5 +570,5 @@ extern "C" int b200_token_logprobs(const void* logits, int dtype, size_t ld, int
         ((uintptr_t)top_ids & 3) || ((uintptr_t)top_logprobs & 3)) return B200_EALIGN;
     LpParams p{logits, tokens, logprobs, entropy, top_ids, top_logprobs, device_status_ptr(), ld, V, G, top};
     if (!p.status) return B200_ENOTIMPL;
-    return dtype == B200_F32 ? lp_launch<true>(p, M, stream) : lp_launch<false>(p, M, stream);
+    return dtype == B200_F32 ? lp_choose<true>(p, M, stream) : lp_choose<false>(p, M, stream);
 }
