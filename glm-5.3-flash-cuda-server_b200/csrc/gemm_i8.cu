@@ -13,6 +13,8 @@
 //   warps 4-11  epilogue: two groups of four warps (one per TMEM lane quadrant) take alternate 16-token chunks
 // Where the items would leave SMs idle, a cluster of CTAs shares one item (SPLIT): each takes a part of K, leaves its sums in its own
 // shared memory, and adds and writes its share of the tokens over distributed shared memory; two CTAs per SM.
+// Behind the quantiser of its own call (`early`) a kernel starts when every CTA of the quantiser has returned from its dependency wait:
+// all that ran before has ended then, so the weights are loaded, and TMEM is taken, while the quantiser still runs.
 // Rows past N or M and columns past K come as zero from the tensor maps.  Every wait is bounded (tma_pipe.cuh).
 #include "b200_internal.h"
 #include "umma_mxf4.cuh"
@@ -32,7 +34,7 @@ constexpr size_t GI_SMEM = 227 * 1024 - GI_STATIC, GI_SMEM_SPLIT = 113 * 1024 - 
 
 struct GiParams {
     void* y; const float* sw; const float* sx; unsigned int* status;
-    int M, N, nst, NT, n_jobs, total, stages, split, tmem_cols;
+    int M, N, nst, NT, n_jobs, total, stages, split, tmem_cols, early;
 };
 
 __device__ __forceinline__ void gi_store(void* y, size_t o, int acc, float sx, float sw, bool bf16) {
@@ -51,9 +53,9 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int S = p.stages, NT = p.NT;
     const uint32_t slot = GI_A_BYTES + (uint32_t)NT * 128u;
-    // TMEM is taken after the kernel before has ended and before the kernel after may start: a kernel that held the columns
-    // while it waits for another that wants them on the same SM would wait for good.
-    pdl_wait();
+    // TMEM is taken after the kernel before has ended (`early`: one that takes none is left) and before the kernel after may start: a
+    // kernel that held the columns while it waits for another that wants them on the same SM would wait for good.
+    if (!p.early) pdl_wait();
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_base_s)), "r"(p.tmem_cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
@@ -76,15 +78,27 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
     const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]);
 
     if (warp == 0) {
+        // the first ring round's weights, which wait for nothing
+        const int ahead = min(S, nst);
+        if (elect_one())
+            for (int it = 0; it < ahead; ++it) {
+                mbar_expect_tx(full0 + it * 8, slot);
+                gx_tma_2d(ring0 + (uint32_t)it * slot, &map_w, (k_first + it) * 128, first / p.n_jobs * 128, full0 + it * 8);
+            }
+        __syncwarp();
+        if (p.early) pdl_wait();
         int s = 0; uint32_t ph = 1;
         for (int i = 0; i < n_items; ++i) {
             const int q = first + i * stride, tile = q / p.n_jobs, job = q - tile * p.n_jobs;
             for (int it = 0; it < nst; ++it) {
-                mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
+                const bool there = i == 0 && it < ahead;
+                if (!there) mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
                 if (elect_one()) {
                     const uint32_t bar = full0 + s * 8, dst = ring0 + (uint32_t)s * slot;
-                    mbar_expect_tx(bar, slot);
-                    gx_tma_2d(dst, &map_w, (k_first + it) * 128, tile * 128, bar);
+                    if (!there) {
+                        mbar_expect_tx(bar, slot);
+                        gx_tma_2d(dst, &map_w, (k_first + it) * 128, tile * 128, bar);
+                    }
                     gx_tma_2d(dst + GI_A_BYTES, &map_x, (k_first + it) * 128, job * NT, bar);
                 }
                 __syncwarp();
@@ -126,6 +140,7 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
     } else if (warp >= 4) {
         const int te = tid - 128, grp = te >> 7, q4 = warp & 3;
         const uint32_t tq = tmem + ((uint32_t)(q4 * 32) << 16);
+        if (p.early) pdl_wait();                       // the tokens' scales
         for (int i = 0; i < n_items; ++i) {
             const int q = first + i * stride, tile = q / p.n_jobs, m0 = (q - tile * p.n_jobs) * NT, rows = min(NT, p.M - m0);
             const int buf = i & 1, row = tile * 128 + q4 * 32 + lane;
@@ -212,7 +227,7 @@ k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUten
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int S = p.stages, NT = p.NT, nst = p.nst, rank = (int)cluster.block_rank();
     const uint32_t slot = GI_A_BYTES + (uint32_t)NT * 64u;
-    pdl_wait();                                        // before TMEM is taken, as above
+    if (!p.early) pdl_wait();                          // before TMEM is taken, as above
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_base_s)), "r"(p.tmem_cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
@@ -234,15 +249,26 @@ k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUten
 
     if (warp == 0) {
         const uint32_t lead0 = gi_mapa(full0, 0);
+        const int ahead = min(S, nst);
+        if (elect_one())
+            for (int it = 0; it < ahead; ++it) {
+                if (rank == 0) mbar_expect_tx(full0 + it * 8, 2 * slot);             // of both CTAs
+                gi_tma_pair(ring0 + (uint32_t)it * slot, &map_w, it * 128, first / p.n_jobs * 256 + rank * 128, lead0 + it * 8);
+            }
+        __syncwarp();
+        if (p.early) pdl_wait();
         int s = 0; uint32_t ph = 1;
         for (int i = 0; i < n_items; ++i) {
             const int q = first + i * stride, tile = q / p.n_jobs, job = q - tile * p.n_jobs;
             for (int it = 0; it < nst; ++it) {
-                mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
+                const bool there = i == 0 && it < ahead;
+                if (!there) mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
                 if (elect_one()) {
                     const uint32_t bar = lead0 + s * 8, dst = ring0 + (uint32_t)s * slot;
-                    if (rank == 0) mbar_expect_tx(full0 + s * 8, 2 * slot);          // of both CTAs
-                    gi_tma_pair(dst, &map_w, it * 128, tile * 256 + rank * 128, bar);
+                    if (!there) {
+                        if (rank == 0) mbar_expect_tx(full0 + s * 8, 2 * slot);
+                        gi_tma_pair(dst, &map_w, it * 128, tile * 256 + rank * 128, bar);
+                    }
                     gi_tma_pair(dst + GI_A_BYTES, &map_x, it * 128, job * NT + rank * (NT / 2), bar);
                 }
                 __syncwarp();
@@ -284,6 +310,7 @@ k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUten
         const int te = tid - 128, grp = te >> 7, q4 = warp & 3;
         const uint32_t tq = tmem + ((uint32_t)(q4 * 32) << 16);
         const uint32_t done = gi_mapa(smem_u32(&acc_empty[0]), 0);
+        if (p.early) pdl_wait();                       // the tokens' scales
         for (int i = 0; i < n_items; ++i) {
             const int q = first + i * stride, tile = q / p.n_jobs, m0 = (q - tile * p.n_jobs) * NT, rows = min(NT, p.M - m0);
             const int buf = i & 1, row = tile * 256 + rank * 128 + q4 * 32 + lane;
@@ -374,8 +401,10 @@ static int gi_launch(GiParams& p, const b200_i8_rows* W, const b200_i8_rows* x, 
     return check_launch("k_gemm_i8");
 }
 
-int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows* x, int M, int N, int K, cudaStream_t s) {
+// early: the launch before on the stream is the quantiser of x, which releases its dependents after its own dependency wait.
+int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows* x, int M, int N, int K, int early, cudaStream_t s) {
     GiParams p{};
+    p.early = early;
     p.y = y; p.sw = W->scale; p.sx = x->scale; p.status = device_status_ptr();
     if (!p.status || !tmap_available()) return B200_ENOTIMPL;
     p.M = M; p.N = N; p.nst = (K + 127) / 128;

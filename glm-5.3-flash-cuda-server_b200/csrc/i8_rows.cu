@@ -29,8 +29,9 @@ k_i8_quantize(const void* __restrict__ xin, size_t ldx, int K, int8_t* __restric
     __shared__ uint32_t red[I8Q_THREADS / 32];
     const int tid = threadIdx.x;
     const size_t row = blockIdx.x, pitch = i8_pitch(K);
-    pdl_launch_dependents();
+    // In this order: what starts now starts after all that came before this launch has ended (gemm_i8.cu relies on it).
     pdl_wait();
+    pdl_launch_dependents();
     const char* xr = static_cast<const char*>(xin) + row * ldx * (F32 ? 4 : 2);
     struct Vec { uint32_t u[W]; };
     auto ld = [&](int c, Vec& v) {                     // elements 8c .. 8c + 7, zero past K
@@ -144,6 +145,7 @@ extern "C" int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const v
     if (M > I8_MAX_ROWS || N > I8_MAX_ROWS || K > I8_MAX_K) return B200_ELIMIT;
     if (((uintptr_t)y & (y_dtype == B200_F32 ? 3 : 1)) || ((uintptr_t)W->q & 15) || ((uintptr_t)W->scale & 3)) return B200_EALIGN;
     b200_i8_rows xq;
+    const bool early = x_dtype != B200_I8;
     if (x_dtype == B200_I8) {
         xq = *static_cast<const b200_i8_rows*>(x);
         if (!xq.q || !xq.scale) return B200_EINVAL;
@@ -160,5 +162,5 @@ extern "C" int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const v
         xq = b200_i8_rows{q, scale};
     }
     if (gemv_i8_takes(M, K)) return gemv_i8(y, y_dtype == B200_BF16, W, xq.q, B200_I8, 0, xq.scale, M, N, K, stream);
-    return gemm_i8_wide(y, y_dtype == B200_BF16, W, &xq, M, N, K, stream);
+    return gemm_i8_wide(y, y_dtype == B200_BF16, W, &xq, M, N, K, early, stream);
 }
