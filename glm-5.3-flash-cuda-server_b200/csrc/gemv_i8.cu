@@ -34,6 +34,8 @@ enum { GV_X_F32 = B200_F32, GV_X_BF16 = B200_BF16, GV_X_I8 = B200_I8 };
 template <int XT>
 __device__ __forceinline__ void gv_stage_x(const GvParams& p, int8_t* xs, float* sxs, uint32_t* red, int warp, int lane) {
     const int kp = p.blocks * 64;
+    if (p.M < 8)                                       // the row of zeros
+        for (int i = warp * 32 + lane; i < kp / 16; i += GV_THREADS) *reinterpret_cast<uint4*>(xs + (size_t)p.M * p.xpitch + i * 16) = make_uint4(0u, 0u, 0u, 0u);
     if (XT == GV_X_I8) {
         const int8_t* q = static_cast<const int8_t*>(p.x);
         const int nv = kp / 16;
@@ -136,7 +138,8 @@ k_gemv_i8(const __grid_constant__ GvParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = lane >> 2, kq = (lane & 3) * 16;
     const int b0 = (int)((long long)p.blocks * warp / GV_WARPS), b1 = (int)((long long)p.blocks * (warp + 1) / GV_WARPS);
-    const int chunks = (b1 - b0 + GV_LOADS - 1) / GV_LOADS;
+    const int chunks = max(1, (b1 - b0 + GV_LOADS - 1) / GV_LOADS);
+    const int full = min(b1, (int)(p.pitch >> 6));      // blocks of the slice that lie within the row
     const int n_units = (p.units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     const int steps = n_units * chunks;
     pdl_launch_dependents();
@@ -150,60 +153,67 @@ k_gemv_i8(const __grid_constant__ GvParams p) {
     }
     pdl_wait();
 
-    uint4 wn[GV_LOADS];
+    // Steps: the chunks of GV_LOADS blocks of this warp's slice, unit by unit.  A slice of no blocks has one chunk of zeros.
     int lu = 0, lc = 0;                                // unit and chunk of the next load
-    auto load = [&] {
-        const int n = min(((int)blockIdx.x + lu * (int)gridDim.x) * GV_ROWS + r, p.N - 1);      // rows past N: their sums are not written
-        const int8_t* row = p.w + (size_t)n * p.pitch;
-        const int k0 = (b0 + lc * GV_LOADS) * 64 + kq, k1 = min((size_t)b1 * 64, p.pitch);
-        #pragma unroll
-        for (int i = 0; i < GV_LOADS; ++i) wn[i] = k0 + i * 64 < k1 ? gv_ldw(row + k0 + i * 64) : make_uint4(0u, 0u, 0u, 0u);
+    const int8_t* row = p.w;
+    auto load = [&](uint4 (&w)[GV_LOADS]) {
+        if (lc == 0) row = p.w + (size_t)min(((int)blockIdx.x + lu * (int)gridDim.x) * GV_ROWS + r, p.N - 1) * p.pitch;      // rows past N: their sums are not written
+        const int bl = b0 + lc * GV_LOADS;
+        const int8_t* q = row + (size_t)bl * 64 + kq;
+        if (bl + GV_LOADS <= full) {
+            #pragma unroll
+            for (int i = 0; i < GV_LOADS; ++i) w[i] = gv_ldw(q + i * 64);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < GV_LOADS; ++i)
+                w[i] = bl + i < b1 && (size_t)(bl + i) * 64 + kq < p.pitch ? gv_ldw(q + i * 64) : make_uint4(0u, 0u, 0u, 0u);
+        }
         if (++lc == chunks) { lc = 0; ++lu; }
     };
-    if (steps) load();
+    uint4 wa[GV_LOADS], wb[GV_LOADS];
+    load(wa);
     gv_stage_x<XT>(p, xs, sxs, red, warp, lane);
     __syncthreads();
 
-    const int8_t* xrow = xs + (size_t)r * p.xpitch + kq;
-    const bool mine = r < p.M;
+    // rows past M read a row of zeros
+    const int8_t* xrow = xs + (size_t)min(r, p.M) * p.xpitch + b0 * 64 + kq;
     const int per = p.M * GV_ROWS;                     // outputs of a unit
-    int step = 0;
-    for (int u0 = 0; u0 < n_units; u0 += p.batch) {
-        const int nu = min(p.batch, n_units - u0);
-        for (int u = 0; u < nu; ++u) {
-            int d[4] = {0, 0, 0, 0};
-            for (int c = 0; c < chunks; ++c) {
-                uint4 w[GV_LOADS];
-                #pragma unroll
-                for (int i = 0; i < GV_LOADS; ++i) w[i] = wn[i];
-                if (++step < steps) load();
-                #pragma unroll
-                for (int i = 0; i < GV_LOADS; ++i) {
-                    const int b = b0 + c * GV_LOADS + i;
-                    if (b < b1) {
-                        const uint4 x = mine ? *reinterpret_cast<const uint4*>(xrow + b * 64) : make_uint4(0u, 0u, 0u, 0u);
-                        gv_mma(d, x.x, x.y, w[i].x, w[i].y);
-                        gv_mma(d, x.z, x.w, w[i].z, w[i].w);
-                    }
-                }
-            }
-            // token r, weight rows 2 * (lane & 3) and the next
-            if (mine) *reinterpret_cast<int2*>(&part[(u * GV_WARPS + warp) * per + r * GV_ROWS + 2 * (lane & 3)]) = make_int2(d[0], d[1]);
+    int d[4] = {0, 0, 0, 0}, c = 0, u = 0, u0 = 0;     // chunk; unit of the batch; the batch's first unit
+    auto consume = [&](const uint4 (&w)[GV_LOADS]) {
+        const int8_t* xc = xrow + c * (GV_LOADS * 64);
+        #pragma unroll
+        for (int i = 0; i < GV_LOADS; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(xc + i * 64);
+            gv_mma(d, x.x, x.y, w[i].x, w[i].y);
+            gv_mma(d, x.z, x.w, w[i].z, w[i].w);
         }
+        if (++c < chunks) return;
+        // token r, weight rows 2 * (lane & 3) and the next
+        if (r < p.M) *reinterpret_cast<int2*>(&part[(u * GV_WARPS + warp) * per + r * GV_ROWS + 2 * (lane & 3)]) = make_int2(d[0], d[1]);
+        d[0] = d[1] = c = 0;
+        if (++u < p.batch && u0 + u < n_units) return;
         __syncthreads();
-        for (int i = tid; i < nu * per; i += GV_THREADS) {
-            const int u = i / per, j = i - u * per, m = j / GV_ROWS;
-            const int n = ((int)blockIdx.x + (u0 + u) * (int)gridDim.x) * GV_ROWS + (j - m * GV_ROWS);
+        for (int i = tid; i < u * per; i += GV_THREADS) {
+            const int v = i / per, j = i - v * per, m = j / GV_ROWS;
+            const int n = ((int)blockIdx.x + (u0 + v) * (int)gridDim.x) * GV_ROWS + (j - m * GV_ROWS);
             if (n < p.N) {
                 int acc = 0;
                 #pragma unroll
-                for (int w = 0; w < GV_WARPS; ++w) acc += part[(u * GV_WARPS + w) * per + j];
+                for (int q = 0; q < GV_WARPS; ++q) acc += part[(v * GV_WARPS + q) * per + j];
                 const float f = __fmul_rn(__fmul_rn(__int2float_rn(acc), sxs[m]), p.sw[n]);
                 if (BF16) static_cast<__nv_bfloat16*>(p.y)[(size_t)m * p.N + n] = __float2bfloat16_rn(f);
                 else static_cast<float*>(p.y)[(size_t)m * p.N + n] = f;
             }
         }
         __syncthreads();
+        u0 += u; u = 0;
+    };
+    for (int s = 0; s < steps; s += 2) {
+        if (s + 1 < steps) load(wb);
+        consume(wa);
+        if (s + 1 == steps) break;
+        if (s + 2 < steps) load(wa);
+        consume(wb);
     }
 }
 
@@ -222,10 +232,12 @@ static int gv_launch(const GvParams& p, size_t smem, cudaStream_t s) {
     return check_launch("k_gemv_i8");
 }
 
-static size_t gv_x_bytes(int M, int K) {
+static int gv_xpitch(int K) {
     const int blocks = (K + 63) / 64;
-    return (size_t)M * (blocks * 64 + (blocks % 2 ? 0 : 64));      // an odd multiple of 64: the rows of a load lie in different banks
+    return blocks * 64 + (blocks % 2 ? 0 : 64);        // an odd multiple of 64: the rows of a load lie in different banks
 }
+// The rows, one of zeros, and what the last chunk of a slice may read past the end (and multiplies by zero).
+static size_t gv_x_bytes(int M, int K) { return (size_t)std::min(M + 1, 8) * gv_xpitch(K) + GV_LOADS * 64; }
 
 bool gemv_i8_takes(int M, int K) { return M <= 8 && gv_x_bytes(M, K) <= GV_SMEM; }
 
@@ -235,7 +247,7 @@ int gemv_i8(void* y, int y_bf16, const b200_i8_rows* W, const void* x, int x_dty
     p.y = y; p.w = W->q; p.sw = W->scale; p.x = x; p.sx = sx; p.ldx = ldx; p.pitch = i8_pitch(K);
     p.M = M; p.N = N; p.K = K;
     p.blocks = (K + 63) / 64;
-    p.xpitch = (int)(gv_x_bytes(M, K) / M);
+    p.xpitch = gv_xpitch(K);
     p.units = (N + GV_ROWS - 1) / GV_ROWS;
     p.batch = GV_PART / (GV_WARPS * M * GV_ROWS);
     credit(B200_CREDIT_GEMM, (double)N * K);
