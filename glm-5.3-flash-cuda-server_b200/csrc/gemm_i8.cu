@@ -53,33 +53,26 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int S = p.stages, NT = p.NT;
     const uint32_t slot = GI_A_BYTES + (uint32_t)NT * 128u;
-    // TMEM is taken after the kernel before has ended (`early`: one that takes none is left) and before the kernel after may start: a
-    // kernel that held the columns while it waits for another that wants them on the same SM would wait for good.
-    if (!p.early) pdl_wait();
-    if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_base_s)), "r"(p.tmem_cols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
-    } else if (warp == 1) {
-        if (lane < S) { mbar_init(smem_u32(&full_bar[lane]), 1); mbar_init(smem_u32(&empty_bar[lane]), 1); }
-        if (lane < 2) { mbar_init(smem_u32(&acc_full[lane]), 1); mbar_init(smem_u32(&acc_empty[lane]), 8); }
-        mbar_fence_init();
-    }
-    gx_fence_before();
-    __syncthreads();
-    gx_fence_after();
-    pdl_launch_dependents();
-    const uint32_t tmem = tmem_base_s;
     // SPLIT: one item per cluster, this CTA's part of its K steps; otherwise every gridDim-th item, all of its steps
     const int rank = SPLIT ? (int)cg::this_cluster().block_rank() : 0;
     const int first = SPLIT ? (int)blockIdx.x / p.split : (int)blockIdx.x, stride = SPLIT ? p.total : (int)gridDim.x;
     const int k_first = SPLIT ? p.nst * rank / p.split : 0, nst = SPLIT ? p.nst * (rank + 1) / p.split - k_first : p.nst;
+    if (warp == 1) {
+        if (lane < S) { mbar_init(smem_u32(&full_bar[lane]), 1); mbar_init(smem_u32(&empty_bar[lane]), 1); }
+        if (lane < 2) { mbar_init(smem_u32(&acc_full[lane]), 1); mbar_init(smem_u32(&acc_empty[lane]), 8); }
+        mbar_fence_init();
+    }
+    if (tid == 0) asm volatile("prefetch.tensormap [%0];\n prefetch.tensormap [%1];" :: "l"(&map_w), "l"(&map_x) : "memory");
+    __syncthreads();
+    if (!p.early) pdl_wait();
     const int n_items = (p.total - first + stride - 1) / stride;      // the grid is no larger than the number of items
     const uint32_t pad = (1024u - (smem_u32(smem) & 1023u)) & 1023u, ring0 = smem_u32(smem) + pad;
     const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]);
 
     if (warp == 0) {
-        // the first ring round's weights, which wait for nothing
-        const int ahead = min(S, nst);
+        // The first weights, which do not wait for the activations.  Behind the quantiser a few of them: the whole ring at once keeps the
+        // rows that it reads (12 rows x [12288 x 4096] 14.2 us with all, 14.0 with five, 13.8 with two stages, 14.6 with none).
+        const int ahead = min(p.early ? min(S, 4) : S, nst);
         if (elect_one())
             for (int it = 0; it < ahead; ++it) {
                 mbar_expect_tx(full0 + it * 8, slot);
@@ -111,7 +104,18 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
             mbar_wait_spin(empty0 + s * 8, ph, p.status, 17);
             if (++s == S) { s = 0; ph ^= 1; }
         }
+    } else if (warp == 2) {
+        // TMEM is taken after the kernel before has ended (`early`: one that takes none is left) and before the kernel after may start:
+        // a kernel that held the columns while it waits for another that wants them on the same SM would wait for good.
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_base_s)), "r"(p.tmem_cols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        gx_fence_before();
+        pdl_launch_dependents();
+        asm volatile("bar.arrive 2, 320;" ::: "memory");
     } else if (warp == 1) {
+        named_sync(2, 320);                            // TMEM is there: this warp and the epilogue's
+        gx_fence_after();
+        const uint32_t tmem = tmem_base_s;
         // D s32 (2), A and B s8 (1), both K-major
         const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((128u >> 4) << 24);
         const uint64_t d0 = gx_desc(ring0);
@@ -139,6 +143,9 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
         }
     } else if (warp >= 4) {
         const int te = tid - 128, grp = te >> 7, q4 = warp & 3;
+        named_sync(2, 320);
+        gx_fence_after();
+        const uint32_t tmem = tmem_base_s;
         const uint32_t tq = tmem + ((uint32_t)(q4 * 32) << 16);
         if (p.early) pdl_wait();                       // the tokens' scales
         for (int i = 0; i < n_items; ++i) {
@@ -192,7 +199,7 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
         }
         cluster.sync();
     } else __syncthreads();
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(p.tmem_cols));
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem_base_s), "r"(p.tmem_cols));
 }
 
 // ---- many tokens: two CTAs of a cluster share a tile of 256 weight rows x NT <= 256 tokens (cta_group::2) -------------------
@@ -220,28 +227,23 @@ template <bool BF16>
 __global__ void __launch_bounds__(GI_THREADS, 1) __cluster_dims__(2, 1, 1)
 k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ uint64_t full_bar[GI_MAX_STAGES], empty_bar[GI_MAX_STAGES], acc_full[2], acc_empty[2];
+    __shared__ uint64_t full_bar[GI_MAX_STAGES], empty_bar[GI_MAX_STAGES], acc_full[2], acc_empty[2], peer_tmem;
     __shared__ uint32_t tmem_base_s;
     __shared__ float sxs[2][GI_MAX_NT];
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int S = p.stages, NT = p.NT, nst = p.nst, rank = (int)cluster.block_rank();
     const uint32_t slot = GI_A_BYTES + (uint32_t)NT * 64u;
-    if (!p.early) pdl_wait();                          // before TMEM is taken, as above
-    if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_base_s)), "r"(p.tmem_cols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
-    } else if (warp == 1) {
+    if (warp == 1) {
         if (lane < S) { mbar_init(smem_u32(&full_bar[lane]), 1); mbar_init(smem_u32(&empty_bar[lane]), 1); }
         if (lane < 2) { mbar_init(smem_u32(&acc_full[lane]), 1); mbar_init(smem_u32(&acc_empty[lane]), 16); }
+        if (lane == 0) mbar_init(smem_u32(&peer_tmem), 1);
         mbar_fence_init();
     }
-    gx_fence_before();
+    if (tid == 0) asm volatile("prefetch.tensormap [%0];\n prefetch.tensormap [%1];" :: "l"(&map_w), "l"(&map_x) : "memory");
     __syncwarp();
     cluster.sync();                                    // both CTAs' barriers stand
-    gx_fence_after();
-    pdl_launch_dependents();
-    const uint32_t tmem = tmem_base_s;
+    if (!p.early) pdl_wait();
     const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
     const int n_items = (p.total - first + stride - 1) / stride;
     const uint32_t ring0 = smem_u32(smem) + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
@@ -249,7 +251,7 @@ k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUten
 
     if (warp == 0) {
         const uint32_t lead0 = gi_mapa(full0, 0);
-        const int ahead = min(S, nst);
+        const int ahead = min(p.early ? min(S, 4) : S, nst);
         if (elect_one())
             for (int it = 0; it < ahead; ++it) {
                 if (rank == 0) mbar_expect_tx(full0 + it * 8, 2 * slot);             // of both CTAs
@@ -279,8 +281,20 @@ k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUten
             mbar_wait_spin(empty0 + s * 8, ph, p.status, 17);
             if (++s == S) { s = 0; ph ^= 1; }
         }
+    } else if (warp == 2) {                            // as above
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&tmem_base_s)), "r"(p.tmem_cols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        gx_fence_before();
+        pdl_launch_dependents();
+        if (rank && lane == 0) gi_arrive_remote(gi_mapa(smem_u32(&peer_tmem), 0));
+        __syncwarp();
+        asm volatile("bar.arrive 2, 320;" ::: "memory");
     } else if (warp == 1) {
+        named_sync(2, 320);
+        gx_fence_after();
+        const uint32_t tmem = tmem_base_s;
         if (rank == 0) {
+            mbar_wait_spin(smem_u32(&peer_tmem), 0, p.status, 31);      // the other CTA has its columns
             const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((256u >> 4) << 24);
             const uint64_t d0 = gx_desc(ring0);
             int s = 0; uint32_t ph = 0;
@@ -308,6 +322,9 @@ k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUten
         }
     } else if (warp >= 4) {
         const int te = tid - 128, grp = te >> 7, q4 = warp & 3;
+        named_sync(2, 320);
+        gx_fence_after();
+        const uint32_t tmem = tmem_base_s;
         const uint32_t tq = tmem + ((uint32_t)(q4 * 32) << 16);
         const uint32_t done = gi_mapa(smem_u32(&acc_empty[0]), 0);
         if (p.early) pdl_wait();                       // the tokens' scales
@@ -340,7 +357,7 @@ k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUten
     gx_fence_before();
     __syncwarp();
     cluster.sync();                                    // nothing of the other CTA's is under way to this one any more
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(p.tmem_cols));
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem_base_s), "r"(p.tmem_cols));
 }
 
 template <bool BF16>
@@ -419,8 +436,21 @@ int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows*
     // More than one tile of tokens: a pair of CTAs per tile.  [12288 x 4096] 2048 rows 80.6 us with single CTAs, 70.0 in pairs;
     // 301 rows x [8192 x 4096] 15.4 and 14.3; 777 rows x [5003 x 2051] 24.4 and 21.0.
     if (M > 128) {
-        p.NT = (p.NT + 31) & ~31;
-        p.total = (N + 255) / 256 * p.n_jobs;
+        const int tiles = (N + 255) / 256, pairs = sm_count() / 2;
+        // Tokens per tile: what takes the fewest clocks by this estimate.  A step of 128 k is 2 NT clocks of MMA, or as long as an SM takes
+        // to bring its part of the tile at 60 B per clock; an item has about 1000 clocks of its own.  777 rows x [5003 x 2051]: four
+        // tiles of 224 tokens are 80 items for 74 pairs, seven of 128 are 140, QA and QB us; 512 rows x [12288 x 4096]: two of 256
+        // and three of 192, QC and QD.
+        long best = 0;
+        for (int jobs = p.n_jobs, most = (M + 31) / 32; jobs <= most && jobs <= 8 * p.n_jobs; ++jobs) {
+            const int nt = ((M + jobs - 1) / jobs + 31) & ~31;
+            if (nt > GI_MAX_NT) continue;
+            const long waves = ((long)tiles * ((M + nt - 1) / nt) + pairs - 1) / pairs;
+            const long cost = waves * ((long)p.nst * std::max(2 * nt, (16384 + 64 * nt) / 60) + 1000);
+            if (!best || cost < best) { best = cost; p.NT = nt; }
+        }
+        p.n_jobs = (M + p.NT - 1) / p.NT;
+        p.total = tiles * p.n_jobs;
         return y_bf16 ? gi_launch_pair<true>(p, W, x, K, s) : gi_launch_pair<false>(p, W, x, K, s);
     }
     if (p.split > 1) return y_bf16 ? gi_launch<true, true>(p, W, x, K, s) : gi_launch<false, true>(p, W, x, K, s);

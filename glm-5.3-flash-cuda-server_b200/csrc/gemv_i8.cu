@@ -18,14 +18,15 @@ constexpr int GV_WARPS = 8, GV_THREADS = GV_WARPS * 32, GV_ROWS = 8;
 constexpr int GV_LOADS = 8;                        // 64-k blocks a warp loads at once
 constexpr int GV_KEEP = 2;                         // vectors of 8 activations a thread keeps between maximum and codes
 constexpr int GV_PART = 4096;                      // partial sums of a batch of units
-// Activations of a CTA, in bytes of shared memory.  Every CTA brings all of them: [4096 x 12288] 4 rows (50 KB) 14.4 us,
-// 5 rows 15.9, 8 rows 32; gemm_i8.cu takes 12.9 there.
-constexpr size_t GV_SMEM = 56 * 1024;
+// Activations of a CTA, in bytes of shared memory.  Every CTA brings all of them: codes x [4096 x 12288], 4 rows (60 KB) 12.2 us, 6 rows
+// (84 KB) 21.3, where gemm_i8.cu takes 14.1.  Behind the quantiser, whose end they have to wait for, 2 rows (36 KB) 14.1, 3 rows
+// (48 KB) 15.0, 4 rows 16.3, and 14.9 there.
+constexpr size_t GV_SMEM = 64 * 1024, GV_SMEM_QUANTISED = 48 * 1024;
 
 struct GvParams {
     void* y; const int8_t* w; const float* sw; const void* x; const float* sx;
     size_t ldx, pitch;
-    int M, N, K, blocks, xpitch, units, batch;     // 64-k blocks of a row; bytes between activation rows in shared memory
+    int M, N, K, blocks, xpitch, units, batch, early;      // 64-k blocks of a row; bytes between activation rows in shared memory
 };
 
 enum { GV_X_F32 = B200_F32, GV_X_BF16 = B200_BF16, GV_X_I8 = B200_I8 };
@@ -120,7 +121,7 @@ __device__ __forceinline__ void gv_stage_x(const GvParams& p, int8_t* xs, float*
 
 __device__ __forceinline__ uint4 gv_ldw(const int8_t* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 __device__ __forceinline__ void gv_mma(int (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
@@ -143,16 +144,6 @@ k_gemv_i8(const __grid_constant__ GvParams p) {
     const int n_units = (p.units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     const int steps = n_units * chunks;
     pdl_launch_dependents();
-    // The first weights are asked into L2 while the kernel before still runs.  Nothing is read: L2 is where its writes go, too.
-    // 7.1 -> 6.4 us for one row x [4096 x 4096] in a row of calls; two units instead of one: 6.7.
-    {
-        const int n = (int)blockIdx.x * GV_ROWS + (lane & 7);
-        const int bytes = min((b1 - b0) * 64, (int)p.pitch - b0 * 64);
-        if (lane < 8 && n < p.N && bytes > 0)
-            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p.w + (size_t)n * p.pitch + b0 * 64), "r"(bytes) : "memory");
-    }
-    pdl_wait();
-
     // Steps: the chunks of GV_LOADS blocks of this warp's slice, unit by unit.  A slice of no blocks has one chunk of zeros.
     int lu = 0, lc = 0;                                // unit and chunk of the next load
     const int8_t* row = p.w;
@@ -171,7 +162,17 @@ k_gemv_i8(const __grid_constant__ GvParams p) {
         if (++lc == chunks) { lc = 0; ++lu; }
     };
     uint4 wa[GV_LOADS], wb[GV_LOADS];
+    // The first weights are asked into L2 while the kernel before still runs.  Nothing is read: L2 is where its writes go, too.
+    // 7.1 -> 6.4 us for one row x [4096 x 4096] in a row of calls; two units instead of one: 6.7.  (`early`: below.)
+    if (!p.early) {
+        const int n = (int)blockIdx.x * GV_ROWS + (lane & 7);
+        const int bytes = min((b1 - b0) * 64, (int)p.pitch - b0 * 64);
+        if (lane < 8 && n < p.N && bytes > 0)
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p.w + (size_t)n * p.pitch + b0 * 64), "r"(bytes) : "memory");
+    }
+    if (!p.early) pdl_wait();
     load(wa);
+    if (p.early) pdl_wait();                           // the activations' codes and scales
     gv_stage_x<XT>(p, xs, sxs, red, warp, lane);
     __syncthreads();
 
@@ -239,11 +240,16 @@ static int gv_xpitch(int K) {
 // The rows, one of zeros, and what the last chunk of a slice may read past the end (and multiplies by zero).
 static size_t gv_x_bytes(int M, int K) { return (size_t)std::min(M + 1, 8) * gv_xpitch(K) + GV_LOADS * 64; }
 
-bool gemv_i8_takes(int M, int K) { return M <= 8 && gv_x_bytes(M, K) <= GV_SMEM; }
+// Against the tensor-core kernel, codes x [4096 x 4096], us: 4 rows 5.3 and 7.2, 8 rows 6.2 and 7.2; [12288 x 4096] 10.8 and 13.7, 12.0 and
+// 13.8; but [154880 x 4096] 102.9 and 104.2, 108.8 and 104.9.
+bool gemv_i8_takes(int M, int N, int K, bool early) {
+    return M <= 8 && gv_x_bytes(M, K) <= (early ? GV_SMEM_QUANTISED : GV_SMEM) && (M <= 4 || (size_t)N * K <= ((size_t)1 << 28));
+}
 
 // x: M rows of x_dtype (B200_F32, B200_BF16 with ldx; B200_I8 with their scales sx).
-int gemv_i8(void* y, int y_bf16, const b200_i8_rows* W, const void* x, int x_dtype, size_t ldx, const float* sx, int M, int N, int K, cudaStream_t s) {
+int gemv_i8(void* y, int y_bf16, const b200_i8_rows* W, const void* x, int x_dtype, size_t ldx, const float* sx, int M, int N, int K, int early, cudaStream_t s) {
     GvParams p{};
+    p.early = early;
     p.y = y; p.w = W->q; p.sw = W->scale; p.x = x; p.sx = sx; p.ldx = ldx; p.pitch = i8_pitch(K);
     p.M = M; p.N = N; p.K = K;
     p.blocks = (K + 63) / 64;

@@ -24,7 +24,7 @@ __device__ __forceinline__ uint32_t i8_codes(float a, float b, float c, float d,
 // weights and prefill chunks (es + 1 bytes per element).
 template <bool F32, bool VEC, int I8Q_THREADS>
 __global__ void __launch_bounds__(I8Q_THREADS)
-k_i8_quantize(const void* __restrict__ xin, size_t ldx, int K, int8_t* __restrict__ q, float* __restrict__ scale) {
+k_i8_quantize(const void* xin, size_t ldx, int K, int8_t* q, float* scale) {
     constexpr int KEEP = F32 ? 4 : 8, W = F32 ? 8 : 4;        // words of 8 elements
     __shared__ uint32_t red[I8Q_THREADS / 32];
     const int tid = threadIdx.x;
@@ -107,9 +107,9 @@ int i8_quantize_launch(const void* x, int x_is_f32, size_t ldx, int rows, int K,
     return check_launch("k_i8_quantize");
 }
 
-// Up to so many bytes of activations the few-row kernel quantises them itself, in every CTA; beyond, in a launch of its own:
-// [4096 x 4096] 1 row 7.1 us and 7.9, 2 rows f32 (32 KB) 9.1 and 9.2, [12288 x 4096] 5 rows bf16 (40 KB) 18.9 and 15.0.
-constexpr size_t I8_GEMV_QUANT_BYTES = 32768;
+// Up to so many activations the few-row kernel quantises them itself, in every CTA; beyond, in a launch of its own.  us with either,
+// bf16: 1 row x [4096 x 4096] 5.9 and 8.2, 4 rows 7.8 and 8.2, 5 rows 10.8 and 9.1; [12288 x 4096] 10.7 and 11.9, 13.3 and 12.8, 16.3 and 13.3.
+constexpr size_t I8_GEMV_QUANT = 16384;
 
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -154,13 +154,13 @@ extern "C" int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const v
         if (int rc = check_x(x, x_dtype, ldx, M, K)) return rc;
         if (!ws) return B200_EINVAL;
         if ((uintptr_t)ws & 255) return B200_EALIGN;
-        if (gemv_i8_takes(M, K) && (size_t)M * K * (x_dtype == B200_F32 ? 4 : 2) <= I8_GEMV_QUANT_BYTES)
-            return gemv_i8(y, y_dtype == B200_BF16, W, x, x_dtype, ldx, nullptr, M, N, K, stream);
+        if (gemv_i8_takes(M, N, K, false) && (size_t)M * K <= I8_GEMV_QUANT)
+            return gemv_i8(y, y_dtype == B200_BF16, W, x, x_dtype, ldx, nullptr, M, N, K, 0, stream);
         int8_t* q = static_cast<int8_t*>(ws);
         float* scale = reinterpret_cast<float*>(q + up256((size_t)M * i8_pitch(K)));
         if (int rc = i8_quantize_launch(x, x_dtype == B200_F32, ldx, M, K, q, scale, stream)) return rc;
         xq = b200_i8_rows{q, scale};
     }
-    if (gemv_i8_takes(M, K)) return gemv_i8(y, y_dtype == B200_BF16, W, xq.q, B200_I8, 0, xq.scale, M, N, K, stream);
+    if (gemv_i8_takes(M, N, K, early)) return gemv_i8(y, y_dtype == B200_BF16, W, xq.q, B200_I8, 0, xq.scale, M, N, K, early, stream);
     return gemm_i8_wide(y, y_dtype == B200_BF16, W, &xq, M, N, K, early, stream);
 }
