@@ -425,34 +425,29 @@ int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows*
     p.y = y; p.sw = W->scale; p.sx = x->scale; p.status = device_status_ptr();
     if (!p.status || !tmap_available()) return B200_ENOTIMPL;
     p.M = M; p.N = N; p.nst = (K + 127) / 128;
-    p.n_jobs = (M + GI_MAX_NT - 1) / GI_MAX_NT;
-    p.NT = ((M + p.n_jobs - 1) / p.n_jobs + 15) & ~15;        // the jobs' tokens evened out: 301 = 160 + 141
-    p.total = (N + 127) / 128 * p.n_jobs;
-    // CTAs per item: as many as one per SM leaves room for.  24 rows x [4096 x 12288], 32 items: 27.2 us with one, 18.0, 14.6 and
-    // 13.3 with 2, 3 and 4; but 16 rows x [12288 x 4096], 96 items: 12.4 with one, 14.0 with 2 on the SMs' second places.
-    p.split = std::max(1, std::min(std::min(sm_count() / p.total, GI_MAX_SPLIT), p.nst / 4));
-    if (p.NT > 128) p.split = 1;                       // the sums would not fit where the operands were
-    credit(B200_CREDIT_GEMM, (double)N * K);
-    // More than one tile of tokens: a pair of CTAs per tile.  [12288 x 4096] 2048 rows 80.6 us with single CTAs, 70.0 in pairs;
-    // 301 rows x [8192 x 4096] 15.4 and 14.3; 777 rows x [5003 x 2051] 24.4 and 21.0.
-    if (M > 128) {
-        const int tiles = (N + 255) / 256, pairs = sm_count() / 2;
-        // Tokens per tile: what takes the fewest clocks by this estimate.  A step of 128 k is 2 NT clocks of MMA, or as long as an SM takes
-        // to bring its part of the tile at 60 B per clock; an item has about 1000 clocks of its own.  777 rows x [5003 x 2051]: four
-        // tiles of 224 tokens are 80 items for 74 pairs, seven of 128 are 140, QA and QB us; 512 rows x [12288 x 4096]: two of 256
-        // and three of 192, QC and QD.
-        long best = 0;
-        for (int jobs = p.n_jobs, most = (M + 31) / 32; jobs <= most && jobs <= 8 * p.n_jobs; ++jobs) {
-            const int nt = ((M + jobs - 1) / jobs + 31) & ~31;
-            if (nt > GI_MAX_NT) continue;
-            const long waves = ((long)tiles * ((M + nt - 1) / nt) + pairs - 1) / pairs;
-            const long cost = waves * ((long)p.nst * std::max(2 * nt, (16384 + 64 * nt) / 60) + 1000);
-            if (!best || cost < best) { best = cost; p.NT = nt; }
+    // Which kernel, and how many tokens per tile: what takes the fewest clocks by this estimate.  A step of 128 k is 2 NT clocks of MMA,
+    // or as long as an SM takes to bring its part of the tile at 60 B per clock; what an item has besides is about 1000 clocks, 2500
+    // for a pair, and the sums that CTAs pass on where they share it (these three fitted to the shapes below and some twenty more).  As many CTAs share an item as one per SM leaves room for: 24 rows x [4096 x 12288], 32 items, 27.2 us with
+    // one, 18.0, 14.6 and 13.3 with 2, 3 and 4; but on the SMs' second places they lose (16 rows x [12288 x 4096], 96 items, 12.4
+    // with one, 14.0 with 2).  Waves: 777 rows x [5003 x 2048], in pairs, four tiles of 224 tokens are 80 items for 74 pairs, 16.8 us,
+    // seven of 128 are 140, 13.5.  Pairs: 2048 rows x [12288 x 4096] 80.6 us with single CTAs, 70.0 in pairs; 301 x [8192 x 4096] 15.4 and
+    // 14.3; 48 x [12288 x 4096] 13.8 and 14.2; shared: 250 x [2000 x 4096] 9.0, in pairs 11.0; 600 x [1000 x 2000] 12.0 and 8.7.
+    const int sms = sm_count(), least = (M + GI_MAX_NT - 1) / GI_MAX_NT;
+    bool pair = false;
+    long best = 0;
+    for (int jobs = least; jobs < least + 8 && (jobs == least || (M + jobs - 1) / jobs > 16); ++jobs) {
+        for (int two = 0; two < 2; ++two) {
+            const int per = (M + jobs - 1) / jobs, nt = two ? (per + 31) & ~31 : (per + 15) & ~15, n_jobs = (M + nt - 1) / nt;
+            const long items = (long)((N + 127) / 128 + two) / (1 + two) * n_jobs, places = sms / (1 + two);
+            // (the sums of an item that is shared lie where its operands were: up to 128 tokens)
+            const int split = two || nt > 128 ? 1 : (int)std::max(1l, std::min({places / items, (long)GI_MAX_SPLIT, (long)p.nst / 4}));
+            const long step = std::max(2 * nt, (int)(GI_A_BYTES + (two ? 64 : 128) * nt) / 60);
+            const long cost = (items * split + places - 1) / places * ((p.nst + split - 1) / split * step + (split > 1 ? 2500 + 25 * nt : two ? 2500 : 1000));
+            if (!best || cost < best) { best = cost; pair = two; p.NT = nt; p.n_jobs = n_jobs; p.total = (int)items; p.split = split; }
         }
-        p.n_jobs = (M + p.NT - 1) / p.NT;
-        p.total = tiles * p.n_jobs;
-        return y_bf16 ? gi_launch_pair<true>(p, W, x, K, s) : gi_launch_pair<false>(p, W, x, K, s);
     }
+    credit(B200_CREDIT_GEMM, (double)N * K);
+    if (pair) return y_bf16 ? gi_launch_pair<true>(p, W, x, K, s) : gi_launch_pair<false>(p, W, x, K, s);
     if (p.split > 1) return y_bf16 ? gi_launch<true, true>(p, W, x, K, s) : gi_launch<false, true>(p, W, x, K, s);
     return y_bf16 ? gi_launch<true, false>(p, W, x, K, s) : gi_launch<false, false>(p, W, x, K, s);
 }
