@@ -32,6 +32,7 @@ namespace cg = cooperative_groups;
 constexpr int LP_LIST = 512;                       // candidates of a CTA
 constexpr int LP_VECS = 4;                         // 16-byte vectors of a tile that a thread has
 constexpr int LP_STAGES = 3;
+constexpr int LP_CLUSTER = 8;                      // CTAs of a row, at most
 constexpr float LP_LOG2E = 1.44269504088896341f, LP_LN2 = 0.693147180559945309f;
 static_assert(B200_LOGPROBS_TOP_MAX <= 32, "a bound is one of 32 maxima");
 
@@ -174,10 +175,12 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     __shared__ uint64_t full_bar[LP_STAGES], empty_bar[LP_STAGES];
     __shared__ unsigned long long vecs[LP_LIST];       // candidates: (ordered maximum, vector)
     __shared__ unsigned long long list[LP_LIST];       // keys
-    __shared__ unsigned long long best[B200_LOGPROBS_TOP_MAX];      // this CTA's, read by the cluster's first CTA
+    __shared__ unsigned long long best[B200_LOGPROBS_TOP_MAX];
     __shared__ uint32_t words[32];
     __shared__ LpStat stats[LP_WARPS];
-    __shared__ LpStat part;                            // this CTA's, read by the cluster's first CTA
+    __shared__ LpStat part;
+    __shared__ unsigned long long all_best[LP_CLUSTER][B200_LOGPROBS_TOP_MAX];      // in the cluster's first CTA: every CTA's
+    __shared__ LpStat all_part[LP_CLUSTER];
     __shared__ int n_vecs, n_list;
     __shared__ unsigned int hist[256];
     __shared__ unsigned int pick[2];
@@ -303,9 +306,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         qs = qt = 0ull;
     };
     settle();
-    auto quickly = [&](const uint4& w) {               // a vector whose elements are all below `quick`
-        float e[NV];
-        lp_unpack<F32>(w, e);
+    auto add = [&](float (&e)[NV]) {                   // elements below st.m, which is `fine`
         const unsigned long long l2 = lp_pack(LP_LOG2E, LP_LOG2E), n2 = lp_pack(-m2, -m2);
         #pragma unroll
         for (int j = 0; j < NV; j += 2) {
@@ -338,7 +339,11 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         const float most = lp_maxof<F32>(lp_maxw<F32>(lp_maxw<F32>(c[0], c[1]), lp_maxw<F32>(c[2], c[3])));
         if (most < quick) {
             #pragma unroll
-            for (int u = 0; u < LP_VECS; ++u) quickly(a[u]);
+            for (int u = 0; u < LP_VECS; ++u) {
+                float e[NV];
+                lp_unpack<F32>(a[u], e);
+                add(e);
+            }
         } else if (!(most < CUDART_INF_F)) st.s = st.t = CUDART_NAN_F;
         else if (most > -CUDART_INF_F) {               // a new maximum, or an equal one: those that equal it are counted, not added
             if (most > st.m) { flush(); raise(most); settle(); }
@@ -347,11 +352,15 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
                 uint4 w = a[0];
                 #pragma unroll
                 for (int i = 1; i < LP_VECS; ++i) if (u == i) w = a[i];
-                #pragma unroll 1
-                for (int j = 0; j < 4; ++j) {
+                float e[NV];
+                lp_unpack<F32>(w, e);
+                #pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    if (e[j] == st.m) { st.n += 1.f; e[j] = -CUDART_INF_F; }
+                if (quick == st.m) add(e);             // `fine`
+                else {
                     #pragma unroll
-                    for (int h = 0; h < NV / 4; ++h) slow(__uint_as_float(F32 ? w.x : h ? w.x & 0xffff0000u : w.x << 16));
-                    w.x = w.y; w.y = w.z; w.z = w.w;
+                    for (int j = 0; j < NV; ++j) slow(e[j]);
                 }
             }
         }
@@ -368,7 +377,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
             }
         }
         if (t + 1 < nt) load(t + 1);
-        if (!((t + 1) & (t + 2)) && t + 2 < nt) {      // tiles 1, 3, 7, ... are done and more than one is left
+        if (!((t + 1) & (t + 2)) && t + 4 < nt) {      // tiles 1, 3, 7, ... are done and more than three are left
             // the CTA's maximum so far for all, at places that do not change from run to run
             const uint32_t most_o = __reduce_max_sync(0xffffffffu, lp_ordered(st.m));
             __syncthreads();
@@ -472,29 +481,27 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
 
     // ---- join the cluster's parts in its first CTA ----
     if (C > 1) {
-        cluster.sync();
-        if (rank == 0) {
-            LpStat all{-CUDART_INF_F, 0.f, 0.f, 0.f};
-            if (warp == 0 && lane < C) all = *cluster.map_shared_rank(&part, lane);
-            if (top) {
-                // no CTA's last one is above the row's top-th
-                unsigned long long least = lane < C ? cluster.map_shared_rank(best, lane)[top - 1] : 0ull;
-                #pragma unroll
-                for (int o = 16; o; o >>= 1) { const unsigned long long q = __shfl_xor_sync(0xffffffffu, least, o); least = q > least ? q : least; }
-                if (tid == 0) n_list = 0;
-                __syncthreads();
-                for (int r = warp; r < C; r += LP_WARPS) {
-                    const unsigned long long k = lane < top ? cluster.map_shared_rank(best, r)[lane] : 0ull;
-                    if (k && k >= least) list[atomicAdd(&n_list, 1)] = k;
-                }
-                __syncthreads();
-                lp_rank<LP_THREADS>(list, n_list, top, best);
-            }
-            if (warp == 0) { all = lp_join(all); if (lane == 0) stats[0] = all; }
-        }
+        __syncthreads();                               // best and part
+        if (tid < top) cluster.map_shared_rank(&all_best[0][0], 0)[rank * B200_LOGPROBS_TOP_MAX + tid] = best[tid];
+        if (tid == 0) { cluster.map_shared_rank(all_part, 0)[rank] = part; n_list = 0; }
         __syncwarp();
-        cluster.barrier_arrive();                      // the other CTAs' shared memory has been read
-        if (rank) { cluster.barrier_wait(); return; }
+        cluster.sync();
+        if (rank) return;
+        if (top) {
+            // no CTA's last one is above the row's top-th
+            unsigned long long least = all_best[0][top - 1];
+            for (int r = 1; r < C; ++r) least = max(least, all_best[r][top - 1]);
+            for (int r = warp; r < C; r += LP_WARPS) {
+                const unsigned long long k = lane < top ? all_best[r][lane] : 0ull;
+                if (k && k >= least) list[atomicAdd(&n_list, 1)] = k;
+            }
+            __syncthreads();
+            lp_rank<LP_THREADS>(list, n_list, top, best);
+        }
+        if (warp == 0) {
+            const LpStat all = lp_join(lane < C ? all_part[lane] : LpStat{-CUDART_INF_F, 0.f, 0.f, 0.f});
+            if (lane == 0) stats[0] = all;
+        }
     } else if (tid == 0) stats[0] = part;
     __syncthreads();
     const LpStat all = stats[0];
@@ -516,7 +523,6 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         p.top_ids[row * top + tid] = bad ? -1 : lp_index(k);
         p.top_lp[row * top + tid] = logp(lp_value(k));
     }
-    if (C > 1) { __syncwarp(); cluster.barrier_wait(); }
 }
 
 template <bool F32, int THREADS>
@@ -546,7 +552,7 @@ static int lp_launch(const LpParams& p, int M, int C, cudaStream_t s) {
 template <bool F32>
 static int lp_choose(const LpParams& p, int M, cudaStream_t s) {
     // CTAs per row: as many as leave the whole batch on the GPU at once (two CTAs per SM), and a tile's worth of work to each.
-    int C = 8;
+    int C = LP_CLUSTER;
     while (C > 1 && ((long long)M * C > 2 * sm_count() || p.V / C < 512 * LP_VECS * LpVec<F32>::N)) C >>= 1;
     // Threads per CTA (1024 per SM in any case): few large CTAs where a row's time counts, small ones, whose barriers cost the others
     // nothing, where there are rows enough.  us with 512 / 256 / 128: [1 x 154880] f32, top 5 10.8 / 12.8 / 17.6; [200 x 20000] f32,
