@@ -15,8 +15,8 @@
 //
 // The likeliest tokens.  Order: logit descending, then index ascending, as one 64-bit key.  A bound is a value that at least `top`
 // elements reach: the top-th of the two largest maxima of every warp.  The first tile gives one, and later elements count only
-// above it (an equal one has a larger index).  Vectors whose maximum counts go to a list in shared memory, and after tiles 1, 3,
-// 7, ... the list gives a higher bound: some 200 vectors of a vocabulary of 154880 in no particular order.  In the end the elements
+// above it (an equal one has a larger index).  Vectors whose maximum counts go to a list in shared memory, and after 1, 4, 16, ...
+// tiles the list gives a higher bound: some 200 vectors of a vocabulary of 154880 in no particular order.  In the end the elements
 // of these vectors that reach the last bound, little more than `top`, are put in order by counting who is larger.  A list that
 // overflows (logits in ascending order; a first tile of masked tokens before many others; thousands of equal logits) is dropped,
 // and the CTA finds the top-th key by radix selection over its part instead.
@@ -76,9 +76,10 @@ __device__ __forceinline__ LpStat lp_join(LpStat a) {
 }
 
 // A bound: the top-th of the largest two (four) k of every one of 16 (8) warps, 0 if there are not so many.  Every thread calls it and gets
-// it; w: 32 words.
+// it.
 template <int LP_THREADS>
-__device__ __noinline__ uint32_t lp_bound(uint32_t k, int top, uint32_t* w) {
+__device__ __noinline__ uint32_t lp_bound(uint32_t k, int top) {
+    __shared__ uint32_t w[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int EACH = 32 / (LP_THREADS / 32);
     uint32_t most[EACH];
@@ -110,11 +111,11 @@ __device__ __noinline__ uint32_t lp_bound(uint32_t k, int top, uint32_t* w) {
 
 // best[0 .. top - 1] <- the largest of list[0 .. n - 1], descending; all keys differ.
 template <int LP_THREADS>
-__device__ __noinline__ void lp_rank(const unsigned long long* list, int n, int top, unsigned long long* best) {
+__device__ __forceinline__ void lp_rank(const unsigned long long (&list)[LP_LIST], int n, int top, unsigned long long (&best)[B200_LOGPROBS_TOP_MAX]) {
     for (int c = threadIdx.x; c < n; c += LP_THREADS) {
         const unsigned long long k = list[c];
         int r = 0;
-        #pragma unroll 8
+        #pragma unroll 4
         for (int i = 0; i < n; ++i) r += list[i] > k;
         if (r < top) best[r] = k;
     }
@@ -176,7 +177,6 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     __shared__ unsigned long long vecs[LP_LIST];       // candidates: (ordered maximum, vector)
     __shared__ unsigned long long list[LP_LIST];       // keys
     __shared__ unsigned long long best[B200_LOGPROBS_TOP_MAX];
-    __shared__ uint32_t words[32];
     __shared__ LpStat stats[LP_WARPS];
     __shared__ LpStat part;
     __shared__ unsigned long long all_best[LP_CLUSTER][B200_LOGPROBS_TOP_MAX];      // in the cluster's first CTA: every CTA's
@@ -217,8 +217,9 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         mbar_expect_tx(smem_u32(&full_bar[s]), bytes);
         bulk_g2s(smem_u32(ring) + s * LP_TILE_BYTES, xv + v0 + t * LP_TILE, bytes, smem_u32(&full_bar[s]));
     };
-    if (tid == 0)
-        for (int t = 0; t < min(nt, LP_STAGES); ++t) request(t);
+    // The first tile alone, the next ones when it has come: three at once from every CTA of a full GPU keep each of them waiting for 28 MB
+    // ([296 x 154880] bf16 25.8 -> 23.8 us).
+    if (tid == 0 && nt) request(0);
     const float sv = si >= 0 ? one(si) : -CUDART_INF_F;
     // this thread's given token, long before its log probability is known
     int token = -1;
@@ -239,6 +240,8 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
             __syncwarp();
         }
         mbar_wait(smem_u32(&full_bar[s]), (uint32_t)(t / LP_STAGES) & 1u, p.status, 30);
+        if (t == 0 && tid == 0)
+            for (int i = 1; i < min(nt, LP_STAGES); ++i) request(i);
         const uint4* q = reinterpret_cast<const uint4*>(ring + (size_t)s * LP_TILE_BYTES) + tid;
         const int left = v1 - v0 - t * LP_TILE;
         if (left >= LP_TILE) {
@@ -266,7 +269,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         #pragma unroll
         for (int j = 0; j < NV; ++j) m = fmaxf(m, v[j]);
     }
-    uint32_t lo = top ? lp_bound<LP_THREADS>(v0 + tid < v1 ? lp_ordered(m) : 0u, top, words) : 0u;
+    uint32_t lo = top ? lp_bound<LP_THREADS>(v0 + tid < v1 ? lp_ordered(m) : 0u, top) : 0u;
     {
         const uint32_t most = __reduce_max_sync(0xffffffffu, lp_ordered(fmaxf(m, sv)));
         if (lane == 0) hist[warp] = most;
@@ -377,7 +380,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
             }
         }
         if (t + 1 < nt) load(t + 1);
-        if (!((t + 1) & (t + 2)) && t + 4 < nt) {      // tiles 1, 3, 7, ... are done and more than three are left
+        if (!(t & (t + 1)) && ((t + 1) & 0x55555555) && t + 4 < nt) {      // 1, 4, 16, ... tiles are done and more than three are left
             // the CTA's maximum so far for all, at places that do not change from run to run
             const uint32_t most_o = __reduce_max_sync(0xffffffffu, lp_ordered(st.m));
             __syncthreads();
@@ -387,7 +390,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
             const float mm = lp_unordered(__reduce_max_sync(0xffffffffu, hist[lane & (LP_WARPS - 1)]));
             if (mm > st.m) { flush(); raise(mm); settle(); }
             if (top && n <= LP_LIST) {
-                const uint32_t b = lp_bound<LP_THREADS>(entry(n), top, words);
+                const uint32_t b = lp_bound<LP_THREADS>(entry(n), top);
                 if (b >= lo && b) { lo = b; bv = lp_unordered(b); held = true; }
             }
         }
@@ -411,7 +414,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     if (top) {
         const int n = n_vecs;
         if (n <= LP_LIST) {
-            lo = max(lo, lp_bound<LP_THREADS>(entry(n), top, words));
+            lo = max(lo, lp_bound<LP_THREADS>(entry(n), top));
             for (int i = tid; i < n; i += LP_THREADS) {
                 if ((uint32_t)(vecs[i] >> 32) < lo) continue;
                 const int q = (int)(uint32_t)vecs[i];
