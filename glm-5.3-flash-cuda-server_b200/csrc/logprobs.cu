@@ -18,8 +18,8 @@
 // above it (an equal one has a larger index).  Vectors whose maximum counts go to a list in shared memory, and after 1, 4, 16, ...
 // tiles the list gives a higher bound: some 200 vectors of a vocabulary of 154880 in no particular order.  In the end the elements
 // of these vectors that reach the last bound, little more than `top`, are put in order by counting who is larger.  A list that
-// overflows (logits in ascending order; a first tile of masked tokens before many others; thousands of equal logits) is dropped,
-// and the CTA finds the top-th key by radix selection over its part instead.
+// overflows (logits in ascending order; a first tile of masked tokens before thousands of others) is dropped, and the CTA
+// finds the top-th key by radix selection over its part instead.
 #include "b200_internal.h"
 #include "tma_pipe.cuh"
 #include <cuda_bf16.h>
@@ -213,7 +213,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
 
     const int nt = (v1 - v0 + LP_TILE - 1) / LP_TILE;
     auto request = [&](int t) {                        // one thread: tile t into its stage
-        const uint32_t bytes = min(LP_TILE_BYTES, (uint32_t)(v1 - v0 - t * LP_TILE) * 16u), s = (uint32_t)t % LP_STAGES;
+        const uint32_t bytes = (uint32_t)min(LP_TILE, v1 - v0 - t * LP_TILE) * 16u, s = (uint32_t)t % LP_STAGES;
         mbar_expect_tx(smem_u32(&full_bar[s]), bytes);
         bulk_g2s(smem_u32(ring) + s * LP_TILE_BYTES, xv + v0 + t * LP_TILE, bytes, smem_u32(&full_bar[s]));
     };
@@ -270,17 +270,17 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         for (int j = 0; j < NV; ++j) m = fmaxf(m, v[j]);
     }
     uint32_t lo = top ? lp_bound<LP_THREADS>(v0 + tid < v1 ? lp_ordered(m) : 0u, top) : 0u;
+    // A bound at the value of a mask would make candidates of all masked elements: if it is the maximum of many threads, what is above
+    // it counts, and if that is too little in the end, the first elements of its value are added.  `held`: `top` elements of earlier
+    // tiles reach the bound.
+    const float low = lp_unordered(lo);
+    bool held = true;
     {
         const uint32_t most = __reduce_max_sync(0xffffffffu, lp_ordered(fmaxf(m, sv)));
         if (lane == 0) hist[warp] = most;
-        __syncthreads();
+        if (__syncthreads_count(lo && v0 + tid < v1 && lp_ordered(m) == lo) > LP_THREADS / 8) { ++lo; held = false; }
         m = lp_unordered(__reduce_max_sync(0xffffffffu, hist[lane & (LP_WARPS - 1)]));
     }
-    // A bound at a mask's value would make candidates of all masked elements.  Then what is above it counts, and if that is too little
-    // in the end, the first masked ones are added: `held` says whether `top` elements of earlier tiles reach the bound.
-    const float lowest = F32 ? -3.402823466e38f : -3.38953139e38f, low = lp_unordered(lo);
-    bool held = true;
-    if (lo && (low == lowest || low == -CUDART_INF_F)) { ++lo; held = false; }
     // nothing to look for: +inf; no bound (fewer than 512 vectors): everything counts
     float bv = !top ? CUDART_INF_F : lo ? lp_unordered(lo) : -CUDART_INF_F;
 
@@ -426,7 +426,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
             }
         }
         __syncthreads();
-        if (n <= LP_LIST && n_list < top) {            // masked ones: no more than top - 1 others are among the first of the part
+        if (n <= LP_LIST && n_list < top) {            // no more than top - 1 are above `low`; if no other element lies below it, the first 64 are enough
             __syncthreads();
             const int i = (rank == 0 ? 0 : head + v0 * NV) + tid;
             if (tid < 2 * B200_LOGPROBS_TOP_MAX && i < (rank == C - 1 ? V : head + v1 * NV)) {

@@ -278,6 +278,33 @@ def test_inputs_that_a_kernel_before_writes_late(M):
         assert same(y, want)
 
 
+def test_two_calls_at_once():
+    """Two streams, each with its own scratch and outputs, the weights shared; kernels that hold tensor memory on both."""
+    P = pkg()
+    x, w = inputs(300, 1500, 1200, 1)
+    W = P.i8_quantize(w.cuda())
+    for Ma, Mb in ((300, 40), (1, 300), (40, 40), (8, 1)):
+        xs = [x[:Ma].cuda(), x[:Mb].cuda()]
+        want = [P.i8_gemm(W, a) for a in xs]
+        ws, ys = [P.i8_gemm_workspace(a.shape[0], 1200, 'cuda') for a in xs], [torch.empty_like(a) for a in want]
+        streams = [torch.cuda.Stream() for _ in xs]
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for a, y, s, st in zip(xs, ys, ws, streams):
+                P.i8_gemm(W, a, y, s, stream=st)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ys, want))
+    assert P.device_status() == 0
+
+
+def test_the_same_rows_as_both_operands():
+    P = pkg()
+    for M in (1, 6, 50, 200):
+        x, _ = inputs(M, 1, 500, M)
+        r = P.i8_quantize(x.cuda())
+        assert same(P.i8_gemm(r, r), product(*rows_of(x), *rows_of(x), torch.float32))
+
+
 def test_many_calls_back_to_back_beside_the_other_kernels():
     """Products of every size between NVFP4 products that hold tensor memory too, twice the same bits."""
     P = pkg()

@@ -119,6 +119,24 @@ def test_masks(V, M, dtype):
     check(x, t, 32)
 
 
+@pytest.mark.parametrize('fill', [-1e4, -65504.0, -1e9, -1e30, -3.3895313892515355e38])
+@pytest.mark.parametrize('V,M', [(20000, 2), (154880, 1), (33333, 600)])
+def test_masks_of_other_values(V, M, fill):
+    """A mask of some large negative value, over whole rows but for a few tokens and over their first half, beside -inf and smaller values."""
+    x, t = make(M, V, M, sd=3.0)
+    g = torch.Generator().manual_seed(7)
+    keep = torch.rand((M, V), generator=g) < 40.0 / V
+    y = torch.where(keep, x, torch.tensor(fill))
+    check(y, t, 32)
+    check(y.to(torch.bfloat16), t, 20)
+    y[:, ::3] = -INF
+    check(y, t, 32)
+    y[:, 1::7] = 2 * fill if fill > -1e38 else fill
+    check(y, t, 20)
+    x[:, :V // 2] = fill
+    check(x, t, 20)
+
+
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('V', [1, 40, 5001, 100003])
 def test_infinities_and_nan(V, dtype):
@@ -253,6 +271,24 @@ def test_captured_replayed_on_another_stream_and_written_late(M):
     late_copy(td, new)
     P.token_logprobs(xd, td, 9, out=out)
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_two_calls_at_once():
+    """Two streams, each with its own outputs, again and again: the calls share nothing."""
+    P = pkg()
+    a, ta = make(40, 30001, 1)
+    b, tb = make(3, 154880, 2, torch.bfloat16)
+    work = [(a.cuda(), ta.cuda(), 7), (b.cuda(), tb.cuda(), 20)]
+    want = [[o.clone() for o in P.token_logprobs(*w)] for w in work]
+    outs = [P.token_logprobs_out(w[1], w[2]) for w in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for w, o, s in zip(work, outs, streams):
+            P.token_logprobs(*w, out=o, stream=s)
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(p, q) for p, q in zip(w, o))
 
 
 def test_scoring_path_from_hidden_rows():
