@@ -368,7 +368,7 @@ class I8Rows:
               'q has to be contiguous int8 [rows, K rounded up to 16]')
         _want(scale.dtype == torch.float32 and scale.is_contiguous() and scale.shape == (q.shape[0],), 'scale has to be contiguous f32 [rows]')
         _device(q, scale)
-        self.q, self.scale, self.N, self.K = q, scale, q.shape[0], K
+        self.q, self.scale, self.N, self.K, self.dev = q, scale, q.shape[0], K, q.get_device()
         self.c = I8RowsC(q.data_ptr(), scale.data_ptr())
         self.ref, self.addr = C.byref(self.c), C.addressof(self.c)
 
@@ -391,8 +391,12 @@ def i8_quantize(x, out=None, stream=None):
         out = I8Rows.empty(M, K, x.device)
     if out.N != M or out.K != K:
         raise B200Error('out has to be I8Rows of the size of x')
-    _device(x, out.q)
-    check(lib().b200_i8_quantize(x.data_ptr(), dt, ld, M, K, out.c.q, out.c.scale, _stream(stream)), 'b200_i8_quantize')
+    dev = torch._C._cuda_getDevice()
+    if x.get_device() != dev or out.dev != dev:
+        raise B200Error('tensors have to be on the current CUDA device')
+    rc = lib().b200_i8_quantize(x.data_ptr(), dt, ld, M, K, out.c.q, out.c.scale, _stream(stream))
+    if rc:
+        check(rc, 'b200_i8_quantize')
     return out
 
 
@@ -404,25 +408,30 @@ def i8_gemm_workspace(M, K, device):
 def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
     """y[M,N] (f32 or bf16) = x[M,K] . W^T in 8-bit integers.  W: I8Rows; x: I8Rows, or f32 / bf16 rows, which are quantised
     within the call, into ws (i8_gemm_workspace(M, K))."""
-    if isinstance(x, I8Rows):
-        M, K, xp, dx, ld, xt, ws, wp = x.N, x.K, x.addr, I8, 0, x.q, x.q, None      # x itself holds what xp points to: it stays bound
+    dev = torch._C._cuda_getDevice()
+    if type(x) is I8Rows:
+        M, K, xp, dx, ld, wp, here = x.N, x.K, x.addr, I8, 0, None, x.dev          # x itself holds what xp points to: it stays bound
     else:
         dx, M, K, ld = _strided_rows(x, 'x')
-        xt, xp = x, x.data_ptr()
+        xp, here = x.data_ptr(), x.get_device()
         if ws is None:
             ws = i8_gemm_workspace(M, K, x.device)
         if ws.nbytes < (M * ((K + 15) & ~15) + 255 & ~255) + (4 * M + 255 & ~255):
             raise B200Error('ws is smaller than i8_gemm_workspace(M, K)')
         wp = ws.data_ptr()
+        if ws.get_device() != here:
+            raise B200Error('tensors have to be on the current CUDA device')
+    N = W.N
     if W.K != K:
         raise B200Error('W and x have to share K')
     if y is None:
-        y = torch.empty((M, W.N), dtype=dtype, device=W.q.device)
-    dy = _DTYPE.get(y.dtype)
-    if dy is None or y.shape != (M, W.N) or not y.is_contiguous():
+        y = torch.empty((M, N), dtype=dtype, device=W.q.device)
+    dy, shape = _DTYPE.get(y.dtype), y.shape
+    if dy is None or len(shape) != 2 or shape[0] != M or shape[1] != N or not y.is_contiguous():
         raise B200Error('y has to be contiguous f32 or bf16 [M, N]')
-    _device(W.q, xt, ws, y)
-    rc = lib().b200_i8_gemm(y.data_ptr(), dy, W.ref, xp, dx, ld, M, W.N, K, wp, _stream(stream))
+    if here != dev or W.dev != dev or y.get_device() != dev:
+        raise B200Error('tensors have to be on the current CUDA device')
+    rc = lib().b200_i8_gemm(y.data_ptr(), dy, W.ref, xp, dx, ld, M, N, K, wp, stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         check(rc, 'b200_i8_gemm')
     return y
@@ -441,8 +450,10 @@ class LogprobsOut(tuple):
                 not (lp.dtype == ent.dtype == tlp.dtype == torch.float32) or
                 not (lp.is_contiguous() and ent.is_contiguous() and ids.is_contiguous() and tlp.is_contiguous())):
             raise B200Error('out has to be token_logprobs_out(tokens, top)')
+        _device(lp, ent, ids, tlp)
         self = cls(tensors)
-        self.size = (M, G, top)
+        self.size, self.dev = (M, G, top), lp.get_device()
+        self.ptrs = lp.data_ptr(), ent.data_ptr(), ids.data_ptr(), tlp.data_ptr()
         return self
 
 
@@ -466,10 +477,11 @@ def token_logprobs(logits, tokens, top=0, out=None, stream=None):
         out = token_logprobs_out(tokens, top)
     elif type(out) is not LogprobsOut or out.size != (M, G, top):
         out = LogprobsOut.of(out, M, G, top)
-    lp, ent, ids, tlp = out
-    _device(logits, tokens, lp, ent, ids, tlp)
-    rc = lib().b200_token_logprobs(logits.data_ptr(), dt, ld, M, V, tokens.data_ptr(), G, lp.data_ptr(), ent.data_ptr(), top, ids.data_ptr(),
-                                   tlp.data_ptr(), _stream(stream))
+    dev = torch._C._cuda_getDevice()
+    if logits.get_device() != dev or tokens.get_device() != dev or out.dev != dev:
+        raise B200Error('tensors have to be on the current CUDA device')
+    lp, ent, ids, tlp = out.ptrs
+    rc = lib().b200_token_logprobs(logits.data_ptr(), dt, ld, M, V, tokens.data_ptr(), G, lp, ent, top, ids, tlp, _stream(stream))
     if rc:
         check(rc, 'b200_token_logprobs')
     return out

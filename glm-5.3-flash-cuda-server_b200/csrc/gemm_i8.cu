@@ -438,6 +438,33 @@ static int gi_launch(GiParams& p, const b200_i8_rows* W, const b200_i8_rows* x, 
     return check_launch("k_gemm_i8");
 }
 
+// Which kernel, and how many tokens per tile: what takes the fewest clocks by this estimate.  A step of 128 k is 2 NT clocks of MMA, or
+// as long as an SM takes to bring its part of the tile at 60 B per clock; what an item has besides is about 1000 clocks, 2500 for a
+// pair, and where CTAs share it also the sums that they pass on (these three fitted to the shapes below and some twenty more).
+//   shared   as many CTAs share an item as one per SM leaves room for: 24 rows x [4096 x 12288], 32 items, 27.2 us with one, 18.0, 14.6
+//            and 13.3 with 2, 3 and 4; but on the SMs' second places they lose (16 rows x [12288 x 4096], 96 items, 12.4 with one, 14.0 with 2)
+//   tiles    777 rows x [5003 x 2048], in pairs: four tiles of 224 tokens are 80 items for 74 pairs, 16.8 us, seven of 128 are 140, 13.5
+//   pairs    2048 rows x [12288 x 4096] 80.6 us with single CTAs, 70.0 in pairs; 301 x [8192 x 4096] 15.4 and 14.3; but 48 x [12288 x
+//            4096] 13.8 and 14.2; 250 x [2000 x 4096] 9.0 shared, 11.0 in pairs; 600 x [1000 x 2000] 12.0 shared, 8.7 in pairs
+struct GiPlan { int M, N, K, pair, NT, n_jobs, total, split; };
+static GiPlan gi_plan(int M, int N, int K) {
+    GiPlan g{M, N, K, 0, 0, 0, 0, 1};
+    const int sms = sm_count(), least = (M + GI_MAX_NT - 1) / GI_MAX_NT, nst = (K + 127) / 128;
+    long best = 0;
+    for (int jobs = least; jobs < least + 8 && (jobs == least || (M + jobs - 1) / jobs > 16); ++jobs) {
+        for (int two = 0; two < 2; ++two) {
+            const int per = (M + jobs - 1) / jobs, nt = two ? (per + 31) & ~31 : (per + 15) & ~15, n_jobs = (M + nt - 1) / nt;
+            const long items = (long)((N + 127) / 128 + two) / (1 + two) * n_jobs, places = sms / (1 + two);
+            // (the sums of an item that is shared lie where its operands were: up to 128 tokens)
+            const int split = two || nt > 128 ? 1 : (int)std::max(1l, std::min({places / items, (long)GI_MAX_SPLIT, (long)nst / 4}));
+            const long step = std::max(2 * nt, (int)(GI_A_BYTES + (two ? 64 : 128) * nt) / 60);
+            const long cost = (items * split + places - 1) / places * ((nst + split - 1) / split * step + (split > 1 ? 2500 + 25 * nt : two ? 2500 : 1000));
+            if (!best || cost < best) { best = cost; g.pair = two; g.NT = nt; g.n_jobs = n_jobs; g.total = (int)items; g.split = split; }
+        }
+    }
+    return g;
+}
+
 // early: the launch before on the stream is the quantiser of x, which releases its dependents after its own dependency wait.
 int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows* x, int M, int N, int K, int early, cudaStream_t s) {
     GiParams p{};
@@ -445,29 +472,13 @@ int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows*
     p.y = y; p.sw = W->scale; p.sx = x->scale; p.status = device_status_ptr();
     if (!p.status || !tmap_available()) return B200_ENOTIMPL;
     p.M = M; p.N = N; p.nst = (K + 127) / 128;
-    // Which kernel, and how many tokens per tile: what takes the fewest clocks by this estimate.  A step of 128 k is 2 NT clocks of MMA,
-    // or as long as an SM takes to bring its part of the tile at 60 B per clock; what an item has besides is about 1000 clocks, 2500
-    // for a pair, and the sums that CTAs pass on where they share it (these three fitted to the shapes below and some twenty more).  As many CTAs share an item as one per SM leaves room for: 24 rows x [4096 x 12288], 32 items, 27.2 us with
-    // one, 18.0, 14.6 and 13.3 with 2, 3 and 4; but on the SMs' second places they lose (16 rows x [12288 x 4096], 96 items, 12.4
-    // with one, 14.0 with 2).  Waves: 777 rows x [5003 x 2048], in pairs, four tiles of 224 tokens are 80 items for 74 pairs, 16.8 us,
-    // seven of 128 are 140, 13.5.  Pairs: 2048 rows x [12288 x 4096] 80.6 us with single CTAs, 70.0 in pairs; 301 x [8192 x 4096] 15.4 and
-    // 14.3; 48 x [12288 x 4096] 13.8 and 14.2; shared: 250 x [2000 x 4096] 9.0, in pairs 11.0; 600 x [1000 x 2000] 12.0 and 8.7.
-    const int sms = sm_count(), least = (M + GI_MAX_NT - 1) / GI_MAX_NT;
-    bool pair = false;
-    long best = 0;
-    for (int jobs = least; jobs < least + 8 && (jobs == least || (M + jobs - 1) / jobs > 16); ++jobs) {
-        for (int two = 0; two < 2; ++two) {
-            const int per = (M + jobs - 1) / jobs, nt = two ? (per + 31) & ~31 : (per + 15) & ~15, n_jobs = (M + nt - 1) / nt;
-            const long items = (long)((N + 127) / 128 + two) / (1 + two) * n_jobs, places = sms / (1 + two);
-            // (the sums of an item that is shared lie where its operands were: up to 128 tokens)
-            const int split = two || nt > 128 ? 1 : (int)std::max(1l, std::min({places / items, (long)GI_MAX_SPLIT, (long)p.nst / 4}));
-            const long step = std::max(2 * nt, (int)(GI_A_BYTES + (two ? 64 : 128) * nt) / 60);
-            const long cost = (items * split + places - 1) / places * ((p.nst + split - 1) / split * step + (split > 1 ? 2500 + 25 * nt : two ? 2500 : 1000));
-            if (!best || cost < best) { best = cost; pair = two; p.NT = nt; p.n_jobs = n_jobs; p.total = (int)items; p.split = split; }
-        }
-    }
+    // The plan depends on the sizes alone; a model has few of them, and the divisions above take a microsecond.
+    static thread_local GiPlan plans[64];
+    GiPlan& g = plans[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 9973u) >> 7 & 63u];
+    if (g.M != M || g.N != N || g.K != K) g = gi_plan(M, N, K);
+    p.NT = g.NT; p.n_jobs = g.n_jobs; p.total = g.total; p.split = g.split;
     credit(B200_CREDIT_GEMM, (double)N * K);
-    if (pair) return y_bf16 ? gi_launch_pair<true>(p, W, x, K, s) : gi_launch_pair<false>(p, W, x, K, s);
+    if (g.pair) return y_bf16 ? gi_launch_pair<true>(p, W, x, K, s) : gi_launch_pair<false>(p, W, x, K, s);
     if (p.split > 1) return y_bf16 ? gi_launch<true, true>(p, W, x, K, s) : gi_launch<false, true>(p, W, x, K, s);
     return y_bf16 ? gi_launch<true, false>(p, W, x, K, s) : gi_launch<false, false>(p, W, x, K, s);
 }

@@ -84,6 +84,8 @@ def test_binding_keeps_what_it_points_to(monkeypatch):
 
     monkeypatch.setattr(b, '_device', lambda *t: None)
     monkeypatch.setattr(b, '_stream', lambda s: None)
+    monkeypatch.setattr(torch._C, '_cuda_getDevice', lambda: -1, raising=False)      # where CPU tensors say they are
+    monkeypatch.setattr(torch._C, '_cuda_getCurrentRawStream', lambda d: 0, raising=False)
     monkeypatch.setattr(b, 'lib', lambda: Fake())
     refs = []
 
