@@ -16,6 +16,10 @@
 // Behind the quantiser of its own call (`early`) a kernel starts when every CTA of the quantiser has returned from its dependency wait:
 // all that ran before has ended then, so the weights are loaded, and TMEM is taken, while the quantiser still runs.
 // Rows past N or M and columns past K come as zero from the tensor maps.  Every wait is bounded (tma_pipe.cuh).
+//
+// Bound by what an SM takes in from L2 (about 43 bytes per clock, 82 GB/s) where the tiles are few, by the weights' stream from HBM where
+// the tokens are (24 rows x [4096 x 12288] 13.9 us, of which 8.9 are the stream at 5.7 TB/s), by the matrix instructions and the power that
+// they draw at 2048 rows ([12288 x 4096] 70 us, 2.94 POP/s, in a short run; 82 us in a long one, where zeros as operands still take 62).
 #include "b200_internal.h"
 #include "umma_mxf4.cuh"
 #include <cuda.h>

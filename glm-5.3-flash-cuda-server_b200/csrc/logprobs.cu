@@ -20,6 +20,10 @@
 // of these vectors that reach the last bound, little more than `top`, are put in order by counting who is larger.  A list that
 // overflows (logits in ascending order; a first tile of masked tokens before thousands of others) is dropped, and the CTA
 // finds the top-th key by radix selection over its part instead.
+//
+// [2048 x 154880] f32 185 us (6.9 TB/s), with 20 alternatives 218; bf16 128 and 172, where the exponential bounds it: 16 a clock and SM are
+// 75 us, and the instructions of an element, about 10 in all, not much less.  [512 x 154880] bf16 42.5 us: 512 rows on 148 SMs are 4 rows
+// on some and 3 on others.  One row of 154880, top 5, 9 us, none of them a unit's limit: a chain of loads, barriers and exchanges.
 #include "b200_internal.h"
 #include "tma_pipe.cuh"
 #include <cuda_bf16.h>
