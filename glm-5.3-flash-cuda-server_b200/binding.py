@@ -344,6 +344,13 @@ def _device(*tensors):
         raise B200Error('tensors have to be on the current CUDA device')
 
 
+def _outputs(tensors, stream):
+    """Outputs that a call on `stream` allocated itself: their memory is not given away before that stream is done with them."""
+    if stream is not None:
+        for t in tensors:
+            t.record_stream(stream)
+
+
 def _strided_rows(x, what):
     """(dtype code, rows, columns, row stride) of a 2-d f32 or bf16 tensor whose rows are contiguous and do not overlap."""
     dt, shape = _DTYPE.get(x.dtype), x.shape
@@ -368,9 +375,13 @@ class I8Rows:
               'q has to be contiguous int8 [rows, K rounded up to 16]')
         _want(scale.dtype == torch.float32 and scale.is_contiguous() and scale.shape == (q.shape[0],), 'scale has to be contiguous f32 [rows]')
         _device(q, scale)
-        self.q, self.scale, self.N, self.K, self.dev = q, scale, q.shape[0], K, q.get_device()
+        self._q, self._scale, self.N, self.K, self.dev = q, scale, q.shape[0], K, q.get_device()
         self.c = I8RowsC(q.data_ptr(), scale.data_ptr())
         self.ref, self.addr = C.byref(self.c), C.addressof(self.c)
+
+    # what `c` points to
+    q = property(lambda self: self._q)
+    scale = property(lambda self: self._scale)
 
     @classmethod
     def empty(cls, rows, K, device):
@@ -389,6 +400,7 @@ def i8_quantize(x, out=None, stream=None):
     if out is None:
         _device(x)
         out = I8Rows.empty(M, K, x.device)
+        _outputs((out.q, out.scale), stream)
     if out.N != M or out.K != K:
         raise B200Error('out has to be I8Rows of the size of x')
     dev = torch._C._cuda_getDevice()
@@ -415,8 +427,9 @@ def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
         dx, M, K, ld = _strided_rows(x, 'x')
         xp, here = x.data_ptr(), x.get_device()
         if ws is None:
-            ws = i8_gemm_workspace(M, K, x.device)
-        if ws.nbytes < (M * ((K + 15) & ~15) + 255 & ~255) + (4 * M + 255 & ~255):
+            with torch.cuda.stream(stream):             # freed on return, so it has to be that stream's
+                ws = i8_gemm_workspace(M, K, x.device)
+        if not ws.is_contiguous() or ws.nbytes < (M * ((K + 15) & ~15) + 255 & ~255) + (4 * M + 255 & ~255):
             raise B200Error('ws is smaller than i8_gemm_workspace(M, K)')
         wp = ws.data_ptr()
         if ws.get_device() != here:
@@ -426,6 +439,7 @@ def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
         raise B200Error('W and x have to share K')
     if y is None:
         y = torch.empty((M, N), dtype=dtype, device=W.q.device)
+        _outputs((y,), stream)
     dy, shape = _DTYPE.get(y.dtype), y.shape
     if dy is None or len(shape) != 2 or shape[0] != M or shape[1] != N or not y.is_contiguous():
         raise B200Error('y has to be contiguous f32 or bf16 [M, N]')
@@ -475,6 +489,7 @@ def token_logprobs(logits, tokens, top=0, out=None, stream=None):
     G = shape[1]
     if out is None:
         out = token_logprobs_out(tokens, top)
+        _outputs(out, stream)
     elif type(out) is not LogprobsOut or out.size != (M, G, top):
         out = LogprobsOut.of(out, M, G, top)
     dev = torch._C._cuda_getDevice()

@@ -240,6 +240,7 @@ int b200_i8_quantize(const void* x, int dtype, size_t ldx, int rows, int K, int8
  *   (b200_i8_gemm_workspace_bytes(M, K) bytes of device memory, 256-byte aligned, used only by this call's kernels).
  * x_dtype B200_I8: x is a HOST pointer to the b200_i8_rows of the activations (b200_i8_quantize: once for several products that
  *   share them); ldx and ws are not used.
+ * y may overlap neither W, x nor ws.
  * Any M, N >= 1 (<= 2^24) and 1 <= K <= 65536.  No counterpart in the reference, whose formats are NVFP4, bf16 and f32. */
 size_t b200_i8_gemm_workspace_bytes(int M, int K);
 int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const void* x, int x_dtype, size_t ldx, int M, int N, int K,

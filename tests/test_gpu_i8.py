@@ -297,6 +297,24 @@ def test_two_calls_at_once():
     assert P.device_status() == 0
 
 
+def test_memory_of_a_call_on_another_stream():
+    """A call on a stream that is busy, with scratch and outputs of its own: what the current stream allocates next shares none of it."""
+    P = pkg()
+    x, w = inputs(300, 500, 1200, 1)
+    W, xd, s = P.i8_quantize(w.cuda()), x.cuda(), torch.cuda.Stream()
+    want = P.i8_gemm(W, xd)
+    sizes = [P.i8_gemm_workspace(300, 1200, 'cuda').nbytes, want.nbytes]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)
+    y = P.i8_gemm(W, xd, stream=s)
+    P.i8_gemm(W, P.i8_quantize(xd, stream=s), stream=s)
+    P.token_logprobs(want, torch.zeros((300, 1), dtype=torch.int32, device='cuda'), 5, stream=s)
+    taken = [torch.zeros(n, dtype=torch.uint8, device='cuda') for n in sizes + [300 * 1200, 1200, 6000] for _ in range(3)]
+    torch.cuda.synchronize()
+    assert same(y, want) and not any(t.any() for t in taken)
+
+
 def test_the_same_rows_as_both_operands():
     P = pkg()
     for M in (1, 6, 50, 200):

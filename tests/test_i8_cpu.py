@@ -96,3 +96,12 @@ def test_binding_keeps_what_it_points_to(monkeypatch):
 
     b.i8_gemm(rows(), rows())
     assert seen == [[True, True]]
+    W = rows()
+    with pytest.raises(AttributeError):
+        W.q = torch.zeros((4, 16), dtype=torch.int8)                                 # the descriptor points to the first one
+    with pytest.raises(AttributeError):
+        W.scale = torch.ones(4)
+    x = torch.zeros(4, 16)
+    for ws in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 20, dtype=torch.uint8)[::2], torch.zeros(100, dtype=torch.uint8)):
+        with pytest.raises(P.B200Error, match='ws'):
+            b.i8_gemm(W, x, ws=ws)
