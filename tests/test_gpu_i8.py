@@ -118,6 +118,38 @@ SHAPES = [(1, 1, 1), (1, 128, 4096), (1, 4096, 256), (2, 7, 17), (3, 130, 31), (
           (1030, 513, 208)]
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('off', range(1, 8))
+def test_rows_at_every_place(off, dtype):
+    """Every distance from a 16-byte boundary, lengths around the vectors that hold a row's ends; NaN around the rows."""
+    P = pkg()
+    for K in (1, 5, 8, 9, 15, 16, 17, 23, 24, 25, 31, 33, 63, 100, 1027, 4090, 4103, 8195, 9001):
+        x, _ = inputs(5, 1, K, 7 * K + off, dtype)
+        for ld in (K, K + 1, K + 3):
+            flat = torch.full((off + 5 * ld + 9,), float('nan'), dtype=dtype, device='cuda')
+            view = flat[off:off + 5 * ld].view(5, ld)[:, :K]
+            view.copy_(x)
+            r, (q, s) = P.i8_quantize(view), rows_of(x)
+            assert np.array_equal(r.q[:, :K].cpu().numpy(), q) and np.array_equal(r.scale.cpu().numpy(), s) and not r.q[:, K:].any()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('M,K,ld', [(601, 1, 1), (297, 64, 64), (330, 100, 104), (1201, 33, 33), (1187, 511, 513), (1190, 1023, 1025), (1500, 512, 515),
+                                    (299, 1024, 1024), (1203, 2047, 2049), (301, 2048, 2048)])
+def test_many_short_rows(M, K, ld, dtype):
+    P = pkg()
+    x, _ = inputs(M, 1, K, M + K, dtype)
+    x[3], x[M - 1, K // 2], x[M - 2, 0], x[M - 3, K - 1] = 0, float('inf'), float('nan'), 1e30
+    big = torch.zeros((M, ld), dtype=dtype, device='cuda')
+    big[:, :K] = x.cuda()
+    pitch = (K + 15) // 16 * 16
+    q, s = torch.full((M + 4, pitch), 77, dtype=torch.int8, device='cuda'), torch.full((M + 4,), 7.0, device='cuda')
+    P.i8_quantize(big[:, :K], out=P.I8Rows(q[:M], s[:M], K))
+    wq, ws = rows_of(x)
+    assert np.array_equal(q[:M, :K].cpu().numpy(), wq) and np.array_equal(s[:M].cpu().numpy(), ws, equal_nan=True)
+    assert not q[:M, K:].any() and (q[M:] == 77).all() and (s[M:] == 7).all()
+
+
 @pytest.mark.parametrize('M,N,K', SHAPES)
 def test_product_is_exact(M, N, K):
     P = pkg()
