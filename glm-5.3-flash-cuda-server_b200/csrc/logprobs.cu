@@ -165,6 +165,16 @@ __device__ __forceinline__ uint32_t lp_maxw(uint32_t a, uint32_t b) {
     else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+// bf16: no element below -1e38, whose exponential is 0 and whose multiple by log2 e is finite (0 * inf would be a NaN).
+template <bool F32>
+__device__ __forceinline__ uint4 lp_finite(uint4 a) {
+    if (!F32) {
+        uint32_t* w = &a.x;
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) asm("max.bf16x2 %0, %0, %1;" : "+r"(w[j]) : "r"(0xfe96fe96u));
+    }
+    return a;
+}
 template <bool F32>
 __device__ __forceinline__ float lp_maxof(uint32_t w) {
     return F32 ? __uint_as_float(w) : lp_max(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -318,7 +328,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
         #pragma unroll
         for (int j = 0; j < NV; j += 2) {
             float2 d = lp_unpack2(lp_fma2(lp_pack(e[j], e[j + 1]), l2, n2));
-            d.x = fmaxf(d.x, -216.f); d.y = fmaxf(d.y, -216.f);
+            if (F32) { d.x = fmaxf(d.x, -216.f); d.y = fmaxf(d.y, -216.f); }
             const unsigned long long f = lp_pack(lp_exp2(d.x), lp_exp2(d.y));
             qs = lp_add2(qs, f); qt = lp_fma2(f, lp_pack(d.x, d.y), qt);
         }
@@ -348,7 +358,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
             #pragma unroll
             for (int u = 0; u < LP_VECS; ++u) {
                 float e[NV];
-                lp_unpack<F32>(a[u], e);
+                lp_unpack<F32>(lp_finite<F32>(a[u]), e);
                 add(e);
             }
         } else if (!(most < CUDART_INF_F)) st.s = st.t = CUDART_NAN_F;
@@ -364,7 +374,11 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
                 #pragma unroll
                 for (int j = 0; j < NV; ++j)
                     if (e[j] == st.m) { st.n += 1.f; e[j] = -CUDART_INF_F; }
-                if (quick == st.m) add(e);             // `fine`
+                if (quick == st.m) {                   // `fine`
+                    #pragma unroll
+                    for (int j = 0; j < NV; ++j) e[j] = fmaxf(e[j], -1e38f);
+                    add(e);
+                }
                 else {
                     #pragma unroll
                     for (int j = 0; j < NV; ++j) slow(e[j]);
