@@ -368,11 +368,11 @@ def _strided_rows(x, what):
 
 
 class I8Rows:
-    """Rows of 8-bit integers, a scale per row: q int8 [rows, pitch] (pitch: K rounded up to 16), scale f32 [rows]."""
+    """Rows of 8-bit integers, a scale per row: q int8 [rows, pitch] (pitch: K rounded up to 32), scale f32 [rows]."""
 
     def __init__(self, q, scale, K):
-        _want(K >= 1 and q.dim() == 2 and q.dtype == torch.int8 and q.is_contiguous() and q.shape[1] == (K + 15) // 16 * 16,
-              'q has to be contiguous int8 [rows, K rounded up to 16]')
+        _want(K >= 1 and q.dim() == 2 and q.dtype == torch.int8 and q.is_contiguous() and q.shape[1] == (K + 31) // 32 * 32,
+              'q has to be contiguous int8 [rows, K rounded up to 32]')
         _want(scale.dtype == torch.float32 and scale.is_contiguous() and scale.shape == (q.shape[0],), 'scale has to be contiguous f32 [rows]')
         _device(q, scale)
         self._q, self._scale, self.N, self.K, self.dev = q, scale, q.shape[0], K, q.get_device()
@@ -386,7 +386,7 @@ class I8Rows:
     @classmethod
     def empty(cls, rows, K, device):
         _want(rows >= 1 and K >= 1, 'rows and K have to be positive')
-        return cls(torch.empty((rows, (K + 15) // 16 * 16), dtype=torch.int8, device=device),
+        return cls(torch.empty((rows, (K + 31) // 32 * 32), dtype=torch.int8, device=device),
                    torch.empty(rows, dtype=torch.float32, device=device), K)
 
     @property
@@ -429,7 +429,7 @@ def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
         if ws is None:
             with torch.cuda.stream(stream):             # freed on return, so it has to be that stream's
                 ws = i8_gemm_workspace(M, K, x.device)
-        if not ws.is_contiguous() or ws.nbytes < (M * ((K + 15) & ~15) + 255 & ~255) + (4 * M + 255 & ~255):
+        if not ws.is_contiguous() or ws.nbytes < (M * ((K + 31) & ~31) + 255 & ~255) + (4 * M + 255 & ~255):
             raise B200Error('ws is smaller than i8_gemm_workspace(M, K)')
         wp = ws.data_ptr()
         if ws.get_device() != here:

@@ -123,7 +123,9 @@ int gemm_f16w_dense(float* y, const b200_wref* W, const void* x, int x_kind, int
 
 // i8_rows.cu: rows of 8-bit integers, one scale per row (the rule stands there).
 constexpr int I8_MAX_K = 65536, I8_MAX_ROWS = 1 << 24;
-__host__ __device__ inline size_t i8_pitch(int K) { return ((size_t)K + 15) & ~(size_t)15; }
+// To whole sectors of 32 bytes: with rows 16 bytes off them a box of a tensor map takes in five per row instead of four (2048 rows x
+// [4096 x 4112] 37.5 us, [4096 x 4128] 31.4; 777 x [5003 x 2051] 16.5 and, 2080 apart, 14.7).
+__host__ __device__ inline size_t i8_pitch(int K) { return ((size_t)K + 31) & ~(size_t)31; }
 int i8_quantize_launch(const void* x, int x_is_f32, size_t ldx, int rows, int K, int8_t* q, float* scale, cudaStream_t s);
 // gemm_i8.cu: y = x . W^T on tcgen05.mma kind::i8, activations already in 8 bits.
 int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows* x, int M, int N, int K, int early, cudaStream_t s);

@@ -76,7 +76,7 @@ k_i8_quantize(const void* xin, size_t ldx, int rows, int K, int8_t* q, float* sc
             }
         }
     };
-    const int end = tid < lo ? tid : hi + tid - lo;    // the first threads take one of those each, five at most
+    const int end = tid < lo ? tid : hi + tid - lo;    // the first threads take one of those each, six at most
     uint32_t ai = 0u;
     auto most = [&](const Vec& v) {                    // over the bits of |x|; bf16 in pairs
         #pragma unroll

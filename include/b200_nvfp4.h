@@ -221,10 +221,11 @@ int b200_dense_mlp(const float* x, const b200_wref* gate, const b200_wref* up, c
  * token); every step is one f32 operation, so that any implementation of the rule gives the same codes:
  *   a = max(max |x[r, :]|, 2^-119)    scale[r] = a / 127    q[r, k] = round_half_to_even(x[r, k] * (127 / a))
  * A row that holds an infinity or a NaN gets a NaN scale and codes of zero, so that its products are NaN.
- * Rows are b200_i8_pitch(K) bytes apart (K rounded up to 16); the bytes past K are written as zero and never used.
+ * Rows are b200_i8_pitch(K) bytes apart (K rounded up to 32, the unit that memory is read in);
+ * the bytes past K are written as zero and never used.
  * No counterpart in the reference. */
 typedef struct {
-    const int8_t* q;          /* [rows, b200_i8_pitch(K)], 16-byte aligned */
+    const int8_t* q;          /* [rows, b200_i8_pitch(K)], 16-byte aligned (32 is faster) */
     const float*  scale;      /* [rows] */
 } b200_i8_rows;
 size_t b200_i8_pitch(int K);

@@ -58,7 +58,7 @@ def test_rows_are_the_rule_s(M, K, dtype):
     x, _ = inputs(M, 1, K, M + K, dtype)
     q, s = rows_of(x)
     r = P.i8_quantize(x.cuda())
-    assert r.q.shape == (M, (K + 15) // 16 * 16)
+    assert r.q.shape == (M, (K + 31) // 32 * 32)
     assert np.array_equal(r.q[:, :K].cpu().numpy(), q) and np.array_equal(r.scale.cpu().numpy(), s)
     assert not r.q[:, K:].any()
 
@@ -104,7 +104,7 @@ def test_rows_of_strided_and_unaligned_tensors(dtype, off, ld):
 def test_rows_behind_the_last_stay():
     P = pkg()
     x = torch.randn((5, 33), generator=gen(3)).cuda()
-    q, s = torch.full((7, 48), 77, dtype=torch.int8, device='cuda'), torch.full((7,), 7.0, device='cuda')
+    q, s = torch.full((7, 64), 77, dtype=torch.int8, device='cuda'), torch.full((7,), 7.0, device='cuda')
     out = P.I8Rows(q[:5], s[:5], 33)
     P.i8_quantize(x, out=out)
     assert (q[5:] == 77).all() and (s[5:] == 7).all()
@@ -142,7 +142,7 @@ def test_many_short_rows(M, K, ld, dtype):
     x[3], x[M - 1, K // 2], x[M - 2, 0], x[M - 3, K - 1] = 0, float('inf'), float('nan'), 1e30
     big = torch.zeros((M, ld), dtype=dtype, device='cuda')
     big[:, :K] = x.cuda()
-    pitch = (K + 15) // 16 * 16
+    pitch = (K + 31) // 32 * 32
     q, s = torch.full((M + 4, pitch), 77, dtype=torch.int8, device='cuda'), torch.full((M + 4,), 7.0, device='cuda')
     P.i8_quantize(big[:, :K], out=P.I8Rows(q[:M], s[:M], K))
     wq, ws = rows_of(x)

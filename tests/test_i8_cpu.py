@@ -12,10 +12,10 @@ PTR = 1 << 20                                               # an address that is
 
 def test_pitch_and_workspace():
     L = pkg().lib()
-    assert [L.b200_i8_pitch(k) for k in (-1, 0, 1, 16, 17, 4096)] == [0, 0, 16, 16, 32, 4096]
+    assert [L.b200_i8_pitch(k) for k in (-1, 0, 1, 32, 17, 4096)] == [0, 0, 32, 32, 32, 4096]
     for M, K in ((1, 1), (5, 2051), (2048, 4096)):
         n = L.b200_i8_gemm_workspace_bytes(M, K)
-        assert n % 256 == 0 and n >= M * ((K + 15) // 16 * 16 + 4)
+        assert n % 256 == 0 and n >= M * ((K + 31) // 32 * 32 + 4)
     assert L.b200_i8_gemm_workspace_bytes(1 << 24, 65536) > 1 << 40      # no 32-bit product
 
 
@@ -60,9 +60,9 @@ def test_binding_refuses():
     with pytest.raises(P.B200Error, match='current CUDA device'):
         P.i8_quantize(torch.zeros(4, 8))
     with pytest.raises(P.B200Error):
-        P.I8Rows(torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4), 8)             # rows are 16 bytes apart
+        P.I8Rows(torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4), 8)             # rows are 32 bytes apart
     with pytest.raises(P.B200Error):
-        P.I8Rows(torch.zeros(4, 16, dtype=torch.int8), torch.zeros(5), 8)
+        P.I8Rows(torch.zeros(4, 32, dtype=torch.int8), torch.zeros(5), 8)
     with pytest.raises(P.B200Error):
         P.I8Rows.empty(0, 8, 'cpu')
 
@@ -90,7 +90,7 @@ def test_binding_keeps_what_it_points_to(monkeypatch):
     refs = []
 
     def rows():
-        r = P.I8Rows(torch.zeros((4, 16), dtype=torch.int8), torch.zeros(4), 16)
+        r = P.I8Rows(torch.zeros((4, 32), dtype=torch.int8), torch.zeros(4), 16)
         refs.append(weakref.ref(r))
         return r
 
@@ -98,7 +98,7 @@ def test_binding_keeps_what_it_points_to(monkeypatch):
     assert seen == [[True, True]]
     W = rows()
     with pytest.raises(AttributeError):
-        W.q = torch.zeros((4, 16), dtype=torch.int8)                                 # the descriptor points to the first one
+        W.q = torch.zeros((4, 32), dtype=torch.int8)                                 # the descriptor points to the first one
     with pytest.raises(AttributeError):
         W.scale = torch.ones(4)
     x = torch.zeros(4, 16)
