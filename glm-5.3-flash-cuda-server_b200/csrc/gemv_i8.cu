@@ -172,6 +172,9 @@ k_gemv_i8(const __grid_constant__ GvParams p) {
         if (lane < 8 && n < p.N && bytes > 0)
             asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p.w + (size_t)n * p.pitch + b0 * 64), "r"(bytes) : "memory");
     }
+    // The scales of the units too, which are wanted last (one row x [4096 x 12288] 10.2 -> 9.95 us, [4096 x 4096] 5.1 -> 5.0).
+    for (int i = tid; i < n_units; i += GV_THREADS)
+        asm volatile("prefetch.global.L2 [%0];" :: "l"(p.sw + ((size_t)blockIdx.x + (size_t)i * gridDim.x) * GV_ROWS));
     if (!p.early) pdl_wait();
     load(wa);
     if (p.early) pdl_wait();                           // the activations' codes and scales

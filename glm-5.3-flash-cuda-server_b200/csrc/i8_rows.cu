@@ -140,9 +140,11 @@ int i8_quantize_launch(const void* x, int x_is_f32, size_t ldx, int rows, int K,
     return check_launch("k_i8_quantize");
 }
 
-// Up to so many activations the few-row kernel quantises them itself, in every CTA; beyond, in a launch of its own.  us with either,
-// bf16: 1 row x [4096 x 4096] 5.9 and 8.2, 4 rows 7.8 and 8.2, 5 rows 10.8 and 9.1; [12288 x 4096] 10.7 and 11.9, 13.3 and 12.8, 16.3 and 13.3.
-constexpr size_t I8_GEMV_QUANT = 16384;
+// Up to so many activations the few-row kernel quantises them itself, in every CTA; beyond, in a launch of its own.  us with either in
+// replays (and for calls from the host, where a launch costs more), bf16: 1 row x [4096 x 4096] 5.9 and 6.8 (6.1 and 8.0), x [4096 x 12288]
+// 11.8 and 12.2, x [4096 x 16384] 16.8 and 15.8; 2 rows x [4096 x 4096] 6.8 and 7.2, x [4096 x 8192] 10.5 and 10.3; 3 rows x [4096 x 4096] 8.5 and
+// 7.5 (8.7 and 8.3); 4 rows x [4096 x 2048] 5.9 and 6.2; 5 rows x [4096 x 1600] 6.8 and 6.2 (7.1 and 7.9).
+static bool i8_gemv_quantises(int M, int K) { return (size_t)M * K <= (M == 1 ? 12288 : 8192); }
 
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -187,7 +189,7 @@ extern "C" int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const v
         if (int rc = check_x(x, x_dtype, ldx, M, K)) return rc;
         if (!ws) return B200_EINVAL;
         if ((uintptr_t)ws & 255) return B200_EALIGN;
-        if (gemv_i8_takes(M, N, K, false) && (size_t)M * K <= I8_GEMV_QUANT)
+        if (gemv_i8_takes(M, N, K, false) && i8_gemv_quantises(M, K))
             return gemv_i8(y, y_dtype == B200_BF16, W, x, x_dtype, ldx, nullptr, M, N, K, 0, stream);
         int8_t* q = static_cast<int8_t*>(ws);
         float* scale = reinterpret_cast<float*>(q + up256((size_t)M * i8_pitch(K)));
