@@ -63,6 +63,11 @@ __device__ __forceinline__ float lp_max(float a, float b) { float r; asm("max.Na
 // d = (x - m) log2 e in two steps, for any finite x and m.  -216 and below: 2^d is zero, d finite.
 __device__ __forceinline__ float lp_d(float x, float m) { return fmaxf((x - m) * LP_LOG2E, -216.f); }
 
+// The two halves of a cluster's barrier.  Shared memory of another CTA may be touched only when that CTA is known to have started: every
+// thread arrives where it starts, and waits, long after all have, before the first store into the first CTA's memory.
+__device__ __forceinline__ void lp_cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void lp_cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
 // The warp's parts as one, in every lane.  Parts without elements have m = -inf, n = s = t = 0; s = NaN marks a row that holds +inf or NaN.
 __device__ __forceinline__ LpStat lp_join(LpStat a) {
     const float m = lp_unordered(__reduce_max_sync(0xffffffffu, lp_ordered(a.m)));
@@ -203,6 +208,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const size_t row = blockIdx.x / C;
     const int V = p.V, top = p.top;
+    if (C > 1) lp_cluster_arrive();
     if (tid == 0) {
         n_vecs = n_list = 0;
         #pragma unroll
@@ -502,6 +508,7 @@ k_token_logprobs(const __grid_constant__ LpParams p) {
 
     // ---- join the cluster's parts in its first CTA ----
     if (C > 1) {
+        lp_cluster_wait();                             // the first CTA has started
         __syncthreads();                               // best and part
         if (tid < top) cluster.map_shared_rank(&all_best[0][0], 0)[rank * B200_LOGPROBS_TOP_MAX + tid] = best[tid];
         if (tid == 0) { cluster.map_shared_rank(all_part, 0)[rank] = part; n_list = 0; }

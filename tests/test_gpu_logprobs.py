@@ -291,6 +291,28 @@ def test_two_calls_at_once():
         assert all(torch.equal(p, q) for p, q in zip(w, o))
 
 
+@pytest.mark.parametrize('M,V,top', [(1, 154880, 5), (3, 154880, 32), (20, 70001, 20), (37, 50257, 0), (70, 40000, 3)])
+def test_rows_shared_by_clusters_beside_busy_multiprocessors(M, V, top):
+    """Rows that several CTAs share, while products of another stream take and leave the places that those CTAs start on."""
+    P = pkg()
+    x, t = make(M, V, M + top)
+    xd, td = x.cuda(), t.cuda()
+    want = [o.clone() for o in check(x, t, top)]
+    g = torch.Generator(device='cuda').manual_seed(3)
+    W = P.i8_quantize((torch.randn((3000, 1024), generator=g, device='cuda') * 0.02).to(torch.bfloat16))
+    rows = [P.i8_quantize(torch.randn((n, 1024), generator=g, device='cuda')) for n in (2, 30, 300)]
+    ys, outs = [torch.empty((r.N, 3000), device='cuda') for r in rows], [P.token_logprobs_out(td, top) for _ in range(30)]
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for o in outs:
+        for r, y in zip(rows, ys):
+            P.i8_gemm(W, r, y, stream=a)
+        P.token_logprobs(xd, td, top, out=o, stream=b)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for o in outs for p, q in zip(o, want))
+    assert P.device_status() == 0
+
+
 def test_scoring_path_from_hidden_rows():
     """As a scorer runs them: hidden rows -> 8-bit vocabulary projection -> log probabilities, greedy choice and perplexity."""
     P = pkg()

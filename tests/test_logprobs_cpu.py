@@ -31,3 +31,22 @@ def test_binding_refuses():
         P.token_logprobs(x, t, 2, out=P.token_logprobs_out(t, 3))
     with pytest.raises(P.B200Error, match='current CUDA device'):
         P.token_logprobs(x, t)
+
+
+def test_clusters_meet_before_they_touch_each_other():
+    """Shared memory of another CTA of a cluster may be touched only once that CTA is known to have started: in every kernel a barrier
+    of the whole cluster comes before the first address in another CTA's memory."""
+    import glob
+    import os
+    import re
+    import __graft_entry__ as G
+    seen = 0
+    for path in glob.glob(os.path.join(G.PKG_DIR, 'csrc', '*.cu')):
+        code = re.sub(r'//[^\n]*', '', open(path).read())
+        for kernel in re.split(r'\b__global__\b', code)[1:]:
+            kernel = re.split(r'\n}', kernel)[0]                                       # up to the kernel's last line
+            remote = re.search(r'map_shared_rank|mapa\(', kernel)
+            if remote:
+                seen += 1
+                assert re.search(r'\w*cluster\w*(\.sync|_wait|\.barrier_wait)\(', kernel[:remote.start()]), (path, kernel[:200])
+    assert seen >= 3
