@@ -160,6 +160,18 @@ def _stream(stream):
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def _empty(stream, shape, dtype, device):
+    """What a call on `stream` allocates itself.  The memory is that stream's: a block of the current stream's could be one that a kernel
+    pending there still uses.  It is not given away either before the current stream, whose owner gets the tensor, is done with it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    here = torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(here)
+    return t
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -344,13 +356,6 @@ def _device(*tensors):
         raise B200Error('tensors have to be on the current CUDA device')
 
 
-def _outputs(tensors, stream):
-    """Outputs that a call on `stream` allocated itself: their memory is not given away before that stream is done with them."""
-    if stream is not None:
-        for t in tensors:
-            t.record_stream(stream)
-
-
 def _strided_rows(x, what):
     """(dtype code, rows, columns, row stride) of a 2-d f32 or bf16 tensor whose rows are contiguous and do not overlap."""
     dt, shape = _DTYPE.get(x.dtype), x.shape
@@ -384,10 +389,9 @@ class I8Rows:
     scale = property(lambda self: self._scale)
 
     @classmethod
-    def empty(cls, rows, K, device):
+    def empty(cls, rows, K, device, stream=None):
         _want(rows >= 1 and K >= 1, 'rows and K have to be positive')
-        return cls(torch.empty((rows, (K + 31) // 32 * 32), dtype=torch.int8, device=device),
-                   torch.empty(rows, dtype=torch.float32, device=device), K)
+        return cls(_empty(stream, (rows, (K + 31) // 32 * 32), torch.int8, device), _empty(stream, (rows,), torch.float32, device), K)
 
     @property
     def nbytes(self):
@@ -399,8 +403,7 @@ def i8_quantize(x, out=None, stream=None):
     dt, M, K, ld = _strided_rows(x, 'x')
     if out is None:
         _device(x)
-        out = I8Rows.empty(M, K, x.device)
-        _outputs((out.q, out.scale), stream)
+        out = I8Rows.empty(M, K, x.device, stream)
     if out.N != M or out.K != K:
         raise B200Error('out has to be I8Rows of the size of x')
     dev = torch._C._cuda_getDevice()
@@ -412,9 +415,9 @@ def i8_quantize(x, out=None, stream=None):
     return out
 
 
-def i8_gemm_workspace(M, K, device):
+def i8_gemm_workspace(M, K, device, stream=None):
     """Scratch for i8_gemm on f32 or bf16 activations: their 8-bit rows."""
-    return torch.empty(lib().b200_i8_gemm_workspace_bytes(M, K), dtype=torch.uint8, device=device)
+    return _empty(stream, lib().b200_i8_gemm_workspace_bytes(M, K), torch.uint8, device)
 
 
 def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
@@ -427,8 +430,7 @@ def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
         dx, M, K, ld = _strided_rows(x, 'x')
         xp, here = x.data_ptr(), x.get_device()
         if ws is None:
-            with torch.cuda.stream(stream):             # freed on return, so it has to be that stream's
-                ws = i8_gemm_workspace(M, K, x.device)
+            ws = i8_gemm_workspace(M, K, x.device, stream)
         if not ws.is_contiguous() or ws.nbytes < (M * ((K + 31) & ~31) + 255 & ~255) + (4 * M + 255 & ~255):
             raise B200Error('ws is smaller than i8_gemm_workspace(M, K)')
         wp = ws.data_ptr()
@@ -438,8 +440,7 @@ def i8_gemm(W, x, y=None, ws=None, dtype=torch.float32, stream=None):
     if W.K != K:
         raise B200Error('W and x have to share K')
     if y is None:
-        y = torch.empty((M, N), dtype=dtype, device=W.q.device)
-        _outputs((y,), stream)
+        y = _empty(stream, (M, N), dtype, W.q.device)
     dy, shape = _DTYPE.get(y.dtype), y.shape
     if dy is None or len(shape) != 2 or shape[0] != M or shape[1] != N or not y.is_contiguous():
         raise B200Error('y has to be contiguous f32 or bf16 [M, N]')
@@ -471,12 +472,12 @@ class LogprobsOut(tuple):
         return self
 
 
-def token_logprobs_out(tokens, top):
+def token_logprobs_out(tokens, top, stream=None):
     """Output buffers of token_logprobs for these tokens."""
     _want(tokens.dim() == 2 and top >= 0, 'tokens has to be [M, G], top not negative')
     M, G = tokens.shape
-    f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=tokens.device)
-    return LogprobsOut.of((f32(M, G), f32(M), torch.empty((M, top), dtype=torch.int32, device=tokens.device), f32(M, top)), M, G, top)
+    new = lambda shape, dtype=torch.float32: _empty(stream, shape, dtype, tokens.device)
+    return LogprobsOut.of((new((M, G)), new((M,)), new((M, top), torch.int32), new((M, top))), M, G, top)
 
 
 def token_logprobs(logits, tokens, top=0, out=None, stream=None):
@@ -488,8 +489,7 @@ def token_logprobs(logits, tokens, top=0, out=None, stream=None):
         raise B200Error('tokens has to be contiguous int32 [M, G]')
     G = shape[1]
     if out is None:
-        out = token_logprobs_out(tokens, top)
-        _outputs(out, stream)
+        out = token_logprobs_out(tokens, top, stream)
     elif type(out) is not LogprobsOut or out.size != (M, G, top):
         out = LogprobsOut.of(out, M, G, top)
     dev = torch._C._cuda_getDevice()

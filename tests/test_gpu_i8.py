@@ -347,6 +347,28 @@ def test_memory_of_a_call_on_another_stream():
     assert same(y, want) and not any(t.any() for t in taken)
 
 
+def test_memory_of_a_call_on_another_stream_that_the_current_one_still_writes():
+    """Tensors of the outputs' sizes, freed while the current stream has still to write them: a call on another stream gets none of them."""
+    P = pkg()
+    x, w = inputs(300, 500, 1200, 1)
+    W, xd, s = P.i8_quantize(w.cuda()), x.cuda(), torch.cuda.Stream()
+    want, X = P.i8_gemm(W, xd), P.i8_quantize(xd)
+    t = torch.zeros((300, 1), dtype=torch.int32, device='cuda')
+    wlp = P.token_logprobs(want, t, 5)
+    torch.cuda.synchronize()
+    sizes = [o.nbytes for o in (want, X.q, X.scale) + wlp] + [P.i8_gemm_workspace(300, 1200, 'cuda').nbytes]
+    old = [torch.zeros(n, dtype=torch.uint8, device='cuda') for n in sizes for _ in range(3)]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(20_000_000)
+    for o in old:
+        o.fill_(255)
+    del old, o
+    y, x8, lp = P.i8_gemm(W, xd, stream=s), P.i8_quantize(xd, stream=s), P.token_logprobs(want, t, 5, stream=s)
+    torch.cuda.synchronize()
+    assert same(y, want) and torch.equal(x8.q, X.q) and torch.equal(x8.scale, X.scale)
+    assert all(torch.equal(a, b) for a, b in zip(lp, wlp))
+
+
 def test_the_same_rows_as_both_operands():
     P = pkg()
     for M in (1, 6, 50, 200):
