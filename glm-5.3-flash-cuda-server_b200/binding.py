@@ -198,9 +198,9 @@ class Nvfp4Weight:
         return self.packed.numel() + self.scale.numel() + 4
 
 
-def split_workspace(M, K, device):
+def split_workspace(M, K, device, stream=None):
     """Scratch for gemm(..., ws=) / gemv_multi(..., ws=): the pre-split activation images."""
-    return torch.empty(lib().b200_nvfp4_split_workspace_bytes(M, K), dtype=torch.uint8, device=device)
+    return _empty(stream, lib().b200_nvfp4_split_workspace_bytes(M, K), torch.uint8, device)
 
 
 def gemm(W, x, y=None, dtype=BF16, stream=None, ws=None):
@@ -214,7 +214,7 @@ def gemm(W, x, y=None, dtype=BF16, stream=None, ws=None):
         N, ref = W.shape[0], WRef(W.data_ptr(), None, None, None)
         dtype = F32 if W.dtype == torch.float32 else BF16
     if y is None:
-        y = torch.empty((M, N), dtype=torch.float32, device=x.device)
+        y = _empty(stream, (M, N), torch.float32, x.device)
     if ws is not None:
         check(lib().b200_nvfp4_gemm_ws(_ptr(y), C.byref(ref), _ptr(x2), M, N, K, dtype, _ptr(ws), _stream(stream)), 'b200_nvfp4_gemm_ws')
     else:
@@ -222,8 +222,8 @@ def gemm(W, x, y=None, dtype=BF16, stream=None, ws=None):
     return y if x.dim() == 2 else y[0]
 
 
-def gemm_bf16_workspace(M, K, device):
-    return torch.empty(lib().b200_nvfp4_gemm_bf16_workspace_bytes(M, K), dtype=torch.uint8, device=device)
+def gemm_bf16_workspace(M, K, device, stream=None):
+    return _empty(stream, lib().b200_nvfp4_gemm_bf16_workspace_bytes(M, K), torch.uint8, device)
 
 
 def gemm_bf16(W, x_bf16, y=None, ws=None, stream=None):
@@ -231,9 +231,9 @@ def gemm_bf16(W, x_bf16, y=None, ws=None, stream=None):
     M, K = x_bf16.shape
     assert W.K == K and x_bf16.dtype == torch.bfloat16
     if y is None:
-        y = torch.empty((M, W.N), dtype=torch.float32, device=x_bf16.device)
+        y = _empty(stream, (M, W.N), torch.float32, x_bf16.device)
     if ws is None:
-        ws = gemm_bf16_workspace(M, K, x_bf16.device)
+        ws = gemm_bf16_workspace(M, K, x_bf16.device, stream)
     ref = W.wref()
     check(lib().b200_nvfp4_gemm_bf16(_ptr(y), C.byref(ref), _ptr(x_bf16), M, W.N, K, _ptr(ws), _stream(stream)), 'b200_nvfp4_gemm_bf16')
     return y
@@ -244,9 +244,9 @@ def gemm_bf16_exact(W, x_bf16, y=None, ws=None, stream=None):
     M, K = x_bf16.shape
     assert W.K == K and x_bf16.dtype == torch.bfloat16
     if y is None:
-        y = torch.empty((M, W.N), dtype=torch.float32, device=x_bf16.device)
+        y = _empty(stream, (M, W.N), torch.float32, x_bf16.device)
     if ws is None:
-        ws = torch.empty(lib().b200_nvfp4_gemm_bf16_exact_workspace_bytes(M, K), dtype=torch.uint8, device=x_bf16.device)
+        ws = _empty(stream, lib().b200_nvfp4_gemm_bf16_exact_workspace_bytes(M, K), torch.uint8, x_bf16.device)
     ref = W.wref()
     check(lib().b200_nvfp4_gemm_bf16_exact(_ptr(y), C.byref(ref), _ptr(x_bf16), M, W.N, K, _ptr(ws), _stream(stream)), 'b200_nvfp4_gemm_bf16_exact')
     return y
@@ -257,16 +257,16 @@ def quantize_tokens(x, stream=None):
     row-major; the library writes it step-major), gs [M]."""
     M, K = x.shape
     dev = x.device
-    packed = torch.empty((M, K // 2), dtype=torch.uint8, device=dev)
-    sfb = torch.empty((K // 256, M, 16), dtype=torch.uint8, device=dev)
-    gs = torch.empty(M, dtype=torch.float32, device=dev)
+    packed = _empty(stream, (M, K // 2), torch.uint8, dev)
+    sfb = _empty(stream, (K // 256, M, 16), torch.uint8, dev)
+    gs = _empty(stream, (M,), torch.float32, dev)
     check(lib().b200_nvfp4_quantize_tokens(_ptr(x), 1 if x.dtype == torch.float32 else 0, M, K, _ptr(packed), _ptr(sfb), _ptr(gs),
                                            _stream(stream)), 'b200_nvfp4_quantize_tokens')
     return packed, sfb.permute(1, 0, 2).reshape(M, K // 16).contiguous(), gs
 
 
-def dense_mlp_workspace(M, hidden, inter, device):
-    return torch.empty(lib().b200_dense_mlp_workspace_bytes(M, hidden, inter), dtype=torch.uint8, device=device)
+def dense_mlp_workspace(M, hidden, inter, device, stream=None):
+    return _empty(stream, lib().b200_dense_mlp_workspace_bytes(M, hidden, inter), torch.uint8, device)
 
 
 def dense_mlp(x, gate, up, down, limit=10.0, y=None, ws=None, stream=None):
@@ -274,9 +274,9 @@ def dense_mlp(x, gate, up, down, limit=10.0, y=None, ws=None, stream=None):
     M, H = x.shape
     I = gate.N
     if y is None:
-        y = torch.empty((M, H), dtype=torch.float32, device=x.device)
+        y = _empty(stream, (M, H), torch.float32, x.device)
     if ws is None:
-        ws = dense_mlp_workspace(M, H, I, x.device)
+        ws = dense_mlp_workspace(M, H, I, x.device, stream)
     g, u, d = gate.wref(), up.wref(), down.wref()
     check(lib().b200_dense_mlp(_ptr(x), C.byref(g), C.byref(u), C.byref(d), H, I, float(limit), _ptr(y), _ptr(ws), M, _stream(stream)),
           'b200_dense_mlp')
@@ -299,7 +299,7 @@ def gemv_multi(weights, xs, M=1, ys=None, stream=None, jobs=None, ws=None):
     if not isinstance(xs, (list, tuple)):
         xs = [xs] * len(weights)
     if ys is None:
-        ys = [torch.empty((M, W.N), dtype=torch.float32, device=xs[0].device) for W in weights]
+        ys = [_empty(stream, (M, W.N), torch.float32, xs[0].device) for W in weights]
     if jobs is None:
         jobs = make_jobs(weights, xs, ys)
     if ws is not None:
@@ -310,13 +310,13 @@ def gemv_multi(weights, xs, M=1, ys=None, stream=None, jobs=None, ws=None):
 
 
 def f32_to_bf16(src, stream=None):
-    dst = torch.empty(src.shape, dtype=torch.bfloat16, device=src.device)
+    dst = _empty(stream, src.shape, torch.bfloat16, src.device)
     check(lib().b200_f32_to_bf16(_ptr(dst), _ptr(src), src.numel(), _stream(stream)), 'b200_f32_to_bf16')
     return dst
 
 
 def bf16_to_f32(src, stream=None):
-    dst = torch.empty(src.shape, dtype=torch.float32, device=src.device)
+    dst = _empty(stream, src.shape, torch.float32, src.device)
     check(lib().b200_bf16_to_f32(_ptr(dst), _ptr(src), src.numel(), _stream(stream)), 'b200_bf16_to_f32')
     return dst
 
@@ -326,16 +326,15 @@ def quantize(w_bf16, gscale_in=None, out=None, stream=None):
     N, K = w_bf16.shape
     dev = w_bf16.device
     if out is None:
-        out = Nvfp4Weight(torch.empty((N, K // 2), dtype=torch.uint8, device=dev),
-                          torch.empty((N, K // 16), dtype=torch.uint8, device=dev),
-                          torch.empty(1, dtype=torch.float32, device=dev), device=dev)
+        out = Nvfp4Weight(_empty(stream, (N, K // 2), torch.uint8, dev), _empty(stream, (N, K // 16), torch.uint8, dev),
+                          _empty(stream, (1,), torch.float32, dev), device=dev)
     check(lib().b200_nvfp4_quantize(_ptr(w_bf16), N, K, _ptr(out.packed), _ptr(out.scale), _ptr(out.gscale),
                                     _ptr(gscale_in), _stream(stream)), 'b200_nvfp4_quantize')
     return out
 
 
 def dequantize(W, stream=None):
-    out = torch.empty((W.N, W.K), dtype=torch.float32, device=W.packed.device)
+    out = _empty(stream, (W.N, W.K), torch.float32, W.packed.device)
     m = W.mat()
     check(lib().b200_nvfp4_dequantize(_ptr(out), C.byref(m), W.N, W.K, _stream(stream)), 'b200_nvfp4_dequantize')
     return out
@@ -531,15 +530,18 @@ class MoeLayer:
         if M not in self._ws:
             n = lib().b200_moe_workspace_bytes(C.byref(self.c), M)
             self._ws[M] = torch.empty(n, dtype=torch.uint8, device=self.router.device)
+            # kept for calls on any stream: whatever used this memory before has to be done with it
+            if self._ws[M].is_cuda and not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
         return self._ws[M]
 
 
 def moe_route(layer, x, stream=None):
     x2 = x if x.dim() == 2 else x.unsqueeze(0)
     M = x2.shape[0]
-    sel = torch.empty((M, layer.topk), dtype=torch.int32, device=x.device)
-    wts = torch.empty((M, layer.topk), dtype=torch.float32, device=x.device)
-    logits = torch.empty((M, layer.n_expert), dtype=torch.float32, device=x.device)
+    sel = _empty(stream, (M, layer.topk), torch.int32, x.device)
+    wts = _empty(stream, (M, layer.topk), torch.float32, x.device)
+    logits = _empty(stream, (M, layer.n_expert), torch.float32, x.device)
     check(lib().b200_moe_route(_ptr(x2), C.byref(layer.c), _ptr(sel), _ptr(wts), _ptr(logits), M, _stream(stream)), 'b200_moe_route')
     return sel, wts, logits
 
@@ -548,9 +550,9 @@ def moe_forward(layer, x, y=None, sel=None, wts=None, stream=None):
     x2 = x if x.dim() == 2 else x.unsqueeze(0)
     M = x2.shape[0]
     dev = x.device
-    y = torch.empty((M, layer.hidden), dtype=torch.float32, device=dev) if y is None else y
-    sel = torch.empty((M, layer.topk), dtype=torch.int32, device=dev) if sel is None else sel
-    wts = torch.empty((M, layer.topk), dtype=torch.float32, device=dev) if wts is None else wts
+    y = _empty(stream, (M, layer.hidden), torch.float32, dev) if y is None else y
+    sel = _empty(stream, (M, layer.topk), torch.int32, dev) if sel is None else sel
+    wts = _empty(stream, (M, layer.topk), torch.float32, dev) if wts is None else wts
     ws = layer.workspace(M)
     check(lib().b200_moe_forward(_ptr(x2), C.byref(layer.c), _ptr(y), _ptr(sel), _ptr(wts), _ptr(ws), M, _stream(stream)), 'b200_moe_forward')
     return y, sel, wts
@@ -573,7 +575,7 @@ def moe_release(layer):
 def moe_experts(layer, x, sel, wts, y=None, stream=None):
     x2 = x if x.dim() == 2 else x.unsqueeze(0)
     M = x2.shape[0]
-    y = torch.empty((M, layer.hidden), dtype=torch.float32, device=x.device) if y is None else y
+    y = _empty(stream, (M, layer.hidden), torch.float32, x.device) if y is None else y
     ws = layer.workspace(M)
     check(lib().b200_moe_experts(_ptr(x2), C.byref(layer.c), _ptr(y), _ptr(sel), _ptr(wts), _ptr(ws), M, _stream(stream)), 'b200_moe_experts')
     return y
@@ -584,9 +586,9 @@ def moe_forward_static(layer, x, y=None, sel=None, wts=None, stream=None):
     x2 = x if x.dim() == 2 else x.unsqueeze(0)
     M = x2.shape[0]
     dev = x.device
-    y = torch.empty((M, layer.hidden), dtype=torch.float32, device=dev) if y is None else y
-    sel = torch.empty((M, layer.topk), dtype=torch.int32, device=dev) if sel is None else sel
-    wts = torch.empty((M, layer.topk), dtype=torch.float32, device=dev) if wts is None else wts
+    y = _empty(stream, (M, layer.hidden), torch.float32, dev) if y is None else y
+    sel = _empty(stream, (M, layer.topk), torch.int32, dev) if sel is None else sel
+    wts = _empty(stream, (M, layer.topk), torch.float32, dev) if wts is None else wts
     check(lib().b200_moe_forward_static(_ptr(x2), C.byref(layer.c), _ptr(y), _ptr(sel), _ptr(wts), M, _stream(stream)),
           'b200_moe_forward_static')
     return y, sel, wts
@@ -611,9 +613,9 @@ class EpContext:
 
     def forward(self, x, y=None, sel=None, wts=None, stream=None):
         T, dev = x.shape[0], x.device
-        y = torch.empty((T, self.router.hidden), dtype=torch.float32, device=dev) if y is None else y
-        sel = torch.empty((T, self.router.topk), dtype=torch.int32, device=dev) if sel is None else sel
-        wts = torch.empty((T, self.router.topk), dtype=torch.float32, device=dev) if wts is None else wts
+        y = _empty(stream, (T, self.router.hidden), torch.float32, dev) if y is None else y
+        sel = _empty(stream, (T, self.router.topk), torch.int32, dev) if sel is None else sel
+        wts = _empty(stream, (T, self.router.topk), torch.float32, dev) if wts is None else wts
         check(lib().b200_ep_forward(self.h, _ptr(x), _ptr(y), _ptr(sel), _ptr(wts), T, _stream(stream)), 'b200_ep_forward')
         return y, sel, wts
 

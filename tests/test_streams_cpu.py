@@ -57,7 +57,36 @@ def rows(b, n, k):
     return b.I8Rows(torch.zeros((n, (k + 31) // 32 * 32), dtype=torch.int8), torch.zeros(n), k)
 
 
+def weight(b, n=32, k=256):
+    return b.Nvfp4Weight(torch.zeros((n, k // 2), dtype=torch.uint8), torch.zeros((n, k // 16), dtype=torch.uint8), torch.ones(1), device='cpu')
+
+
+def layer(b):
+    e = [(weight(b), weight(b), weight(b)) for _ in range(2)]
+    L = b.MoeLayer(torch.zeros((2, 256), dtype=torch.bfloat16), torch.zeros(2), e, None, 1, 256, 32)
+    L._ws[3] = torch.zeros(64, dtype=torch.uint8)                                    # kept from an earlier call
+    return L
+
+
+f32, b16 = lambda: torch.zeros(3, 256), lambda: torch.zeros((3, 256), dtype=torch.bfloat16)
 CALLS = {
+    'gemm': lambda b, s: b.gemm(weight(b), f32(), stream=s),
+    'gemm with scratch': lambda b, s: b.gemm(weight(b), f32(), stream=s, ws=b.split_workspace(3, 256, 'cpu', s)),
+    'gemm of a plain matrix': lambda b, s: b.gemm(b16(), f32(), stream=s),
+    'gemm_bf16': lambda b, s: b.gemm_bf16(weight(b), b16(), stream=s),
+    'gemm_bf16_exact': lambda b, s: b.gemm_bf16_exact(weight(b), b16(), stream=s),
+    'quantize_tokens': lambda b, s: b.quantize_tokens(f32(), stream=s),
+    'dense_mlp': lambda b, s: b.dense_mlp(f32(), weight(b), weight(b), weight(b), stream=s),
+    'gemv_multi': lambda b, s: b.gemv_multi([weight(b), weight(b)], f32(), 3, stream=s),
+    'f32_to_bf16': lambda b, s: b.f32_to_bf16(f32(), stream=s),
+    'bf16_to_f32': lambda b, s: b.bf16_to_f32(b16(), stream=s),
+    'quantize': lambda b, s: b.quantize(b16(), stream=s),
+    'dequantize': lambda b, s: b.dequantize(weight(b), stream=s),
+    'moe_route': lambda b, s: b.moe_route(layer(b), f32(), stream=s),
+    'moe_forward': lambda b, s: b.moe_forward(layer(b), f32(), stream=s),
+    'moe_experts': lambda b, s: b.moe_experts(layer(b), f32(), torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, 1), stream=s),
+    'moe_forward_static': lambda b, s: b.moe_forward_static(layer(b), f32(), stream=s),
+    'EpContext.forward': lambda b, s: b.EpContext(layer(b), layer(b), None, 0, 1, 3).forward(f32(), stream=s),
     'i8_quantize': lambda b, s: b.i8_quantize(torch.zeros(3, 40), stream=s),
     'i8_gemm': lambda b, s: b.i8_gemm(rows(b, 5, 40), torch.zeros(3, 40), stream=s),
     'i8_gemm with scratch': lambda b, s: b.i8_gemm(rows(b, 5, 40), torch.zeros(3, 40), ws=torch.zeros(4096, dtype=torch.uint8), stream=s),
