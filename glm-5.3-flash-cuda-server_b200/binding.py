@@ -260,9 +260,12 @@ def quantize_tokens(x, stream=None):
     packed = _empty(stream, (M, K // 2), torch.uint8, dev)
     sfb = _empty(stream, (K // 256, M, 16), torch.uint8, dev)
     gs = _empty(stream, (M,), torch.float32, dev)
+    scale = _empty(stream, (M, K // 16), torch.uint8, dev)
     check(lib().b200_nvfp4_quantize_tokens(_ptr(x), 1 if x.dtype == torch.float32 else 0, M, K, _ptr(packed), _ptr(sfb), _ptr(gs),
                                            _stream(stream)), 'b200_nvfp4_quantize_tokens')
-    return packed, sfb.permute(1, 0, 2).reshape(M, K // 16).contiguous(), gs
+    with torch.cuda.stream(stream):                     # behind the kernel
+        scale.view(M, K // 256, 16).copy_(sfb.permute(1, 0, 2))
+    return packed, scale, gs
 
 
 def dense_mlp_workspace(M, hidden, inter, device, stream=None):

@@ -27,13 +27,14 @@ def paths(P):
         'gemm_bf16_exact': lambda s: out(P.gemm_bf16_exact(gate, xb, stream=s)),
         'dense_mlp': lambda s: out(P.dense_mlp(x, gate, up, down, stream=s)),
         'gemv_multi': lambda s: out(P.gemv_multi([gate, up], x[:4], 4, stream=s)),
+        'quantize_tokens': lambda s: out(P.quantize_tokens(x, stream=s)),
         'f32_to_bf16': lambda s: out(P.f32_to_bf16(x, stream=s)),
         'quantize': lambda s: [P.quantize(xb, stream=s).packed],
         'dequantize': lambda s: out(P.dequantize(gate, stream=s)),
     }
 
 
-NAMES = ['gemm', 'gemm_bf16', 'gemm_bf16_exact', 'dense_mlp', 'gemv_multi', 'f32_to_bf16', 'quantize', 'dequantize']
+NAMES = ['gemm', 'gemm_bf16', 'gemm_bf16_exact', 'dense_mlp', 'gemv_multi', 'quantize_tokens', 'f32_to_bf16', 'quantize', 'dequantize']
 
 
 def occupy(sizes):

@@ -110,3 +110,15 @@ def hold(calls, call):
 @pytest.mark.parametrize('name', CALLS)
 def test_what_a_call_on_another_stream_allocates(calls, name):
     hold(calls, CALLS[name])
+
+
+def test_codes_of_tokens_are_put_in_order_behind_their_kernel(calls, monkeypatch):
+    """quantize_tokens rearranges what its kernel wrote: on the kernel's stream."""
+    b, made, recorded = calls
+    on, copy = [], torch.Tensor.copy_
+    monkeypatch.setattr(torch.Tensor, 'copy_', lambda t, *a: (on.append(torch.cuda.current_stream()), copy(t, *a))[1])
+    contiguous = torch.Tensor.contiguous
+    monkeypatch.setattr(torch.Tensor, 'contiguous', lambda t, *a: (on.append(torch.cuda.current_stream()), contiguous(t, *a))[1])
+    other = Stream()
+    b.quantize_tokens(torch.zeros(3, 512), stream=other)
+    assert on and all(s is other for s in on)
