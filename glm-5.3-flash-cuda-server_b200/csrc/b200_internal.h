@@ -130,8 +130,7 @@ int i8_quantize_launch(const void* x, int x_is_f32, size_t ldx, int rows, int K,
 // gemm_i8.cu: y = x . W^T on tcgen05.mma kind::i8, activations already in 8 bits.
 int gemm_i8_wide(void* y, int y_bf16, const b200_i8_rows* W, const b200_i8_rows* x, int M, int N, int K, int early, cudaStream_t s);
 // gemv_i8.cu: the same for few rows, also from f32 or bf16 activations, quantised in the kernel.
-bool gemv_i8_takes(int M, int N, int K, bool early);
-int gemv_i8(void* y, int y_bf16, const b200_i8_rows* W, const void* x, int x_dtype, size_t ldx, const float* sx, int M, int N, int K, int early,
-            cudaStream_t s);
+bool gemv_i8_takes(int M, int N, int K, bool quantised);
+int gemv_i8(void* y, int y_bf16, const b200_i8_rows* W, const void* x, int x_dtype, size_t ldx, const float* sx, int M, int N, int K, cudaStream_t s);
 
 }  // namespace b200

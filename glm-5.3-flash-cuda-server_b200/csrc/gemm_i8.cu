@@ -13,8 +13,9 @@
 //   warps 4-11  epilogue: two groups of four warps (one per TMEM lane quadrant) take alternate 16-token chunks
 // Where the items would leave SMs idle, a cluster of CTAs shares one item (SPLIT): each takes a part of K, leaves its sums in its own
 // shared memory, and adds and writes its share of the tokens over distributed shared memory; two CTAs per SM.
-// Behind the quantiser of its own call (`early`) a kernel starts when every CTA of the quantiser has returned from its dependency wait:
-// all that ran before has ended then, so the weights are loaded, and TMEM is taken, while the quantiser still runs.
+// Behind the quantiser of its own call (`early`) a kernel starts when every CTA of the quantiser has returned from its dependency wait.
+// What ran before has ended then, so TMEM is taken while the quantiser still runs.  No input is read before the kernel's own
+// dependency wait, the weights neither: only that wait makes an earlier kernel's writes visible.
 // Rows past N or M and columns past K come as zero from the tensor maps.  Every wait is bounded (tma_pipe.cuh).
 //
 // Bound by what an SM takes in from L2 (about 43 bytes per clock, 82 GB/s) where the tiles are few, by the weights' stream from HBM where
@@ -31,6 +32,7 @@ namespace cg = cooperative_groups;
 
 constexpr int GI_THREADS = 384;
 constexpr int GI_MAX_STAGES = 12;
+constexpr int GI_PREFETCH = 2;                     // K steps asked into L2 behind a quantiser
 constexpr int GI_MAX_NT = 256, GI_MAX_SPLIT = 8;
 constexpr uint32_t GI_A_BYTES = 16384;
 constexpr size_t GI_STATIC = 4096;                 // static shared memory, at most
@@ -40,6 +42,10 @@ struct GiParams {
     void* y; const float* sw; const float* sx; unsigned int* status;
     int M, N, nst, NT, n_jobs, total, stages, split, tmem_cols, early;
 };
+
+__device__ __forceinline__ void gi_prefetch(const void* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" :: "l"(map), "r"(x), "r"(y) : "memory");
+}
 
 __device__ __forceinline__ void gi_store(void* y, size_t o, int acc, float sx, float sw, bool bf16) {
     const float v = __fmul_rn(__fmul_rn(__int2float_rn(acc), sx), sw);
@@ -108,28 +114,24 @@ k_gemm_i8(const __grid_constant__ GiParams p, const __grid_constant__ CUtensorMa
     const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]);
 
     if (warp == 0) {
-        // The first weights, which do not wait for the activations.  Behind the quantiser a few of them: the whole ring at once keeps the
-        // rows that it reads (12 rows x [12288 x 4096] 14.2 us with all, 14.0 with five, 13.8 with two stages, 14.6 with none).
-        const int ahead = min(p.early ? min(S, 4) : S, nst);
-        if (elect_one())
-            for (int it = 0; it < ahead; ++it) {
-                mbar_expect_tx(full0 + it * 8, slot);
-                gx_tma_2d(ring0 + (uint32_t)it * slot, &map_w, (k_first + it) * 128, first / p.n_jobs * 128, full0 + it * 8);
-            }
-        __syncwarp();
-        if (p.early) pdl_wait();
+        // While the quantiser runs the first weights are asked into L2.  Nothing is read: L2 is where an earlier kernel's writes go, too.
+        // (us with 0, 2, 4 and 12 steps: 24 rows x [4096 x 12288] 15.2, 14.8, 14.9, 14.8; 4 rows x [4096 x 12288] 14.0, 13.7, 13.6, 14.0;
+        // 777 x [5003 x 2051] in pairs 18.2, 18.3, 18.3, 18.9; 64 x [4096 x 4096] - , 10.4, 10.5, 10.2.)
+        if (p.early) {
+            if (elect_one())
+                for (int it = 0; it < min(GI_PREFETCH, nst); ++it) gi_prefetch(&map_w, (k_first + it) * 128, first / p.n_jobs * 128);
+            __syncwarp();
+            pdl_wait();
+        }
         int s = 0; uint32_t ph = 1;
         for (int i = 0; i < n_items; ++i) {
             const int q = first + i * stride, tile = q / p.n_jobs, job = q - tile * p.n_jobs;
             for (int it = 0; it < nst; ++it) {
-                const bool there = i == 0 && it < ahead;
-                if (!there) mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
+                mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
                 if (elect_one()) {
                     const uint32_t bar = full0 + s * 8, dst = ring0 + (uint32_t)s * slot;
-                    if (!there) {
-                        mbar_expect_tx(bar, slot);
-                        gx_tma_2d(dst, &map_w, (k_first + it) * 128, tile * 128, bar);
-                    }
+                    mbar_expect_tx(bar, slot);
+                    gx_tma_2d(dst, &map_w, (k_first + it) * 128, tile * 128, bar);
                     gx_tma_2d(dst + GI_A_BYTES, &map_x, (k_first + it) * 128, job * NT, bar);
                 }
                 __syncwarp();
@@ -282,26 +284,21 @@ k_gemm_i8_pair(const __grid_constant__ GiParams p, const __grid_constant__ CUten
 
     if (warp == 0) {
         const uint32_t lead0 = gi_mapa(full0, 0);
-        const int ahead = min(p.early ? min(S, 4) : S, nst);
-        if (elect_one())
-            for (int it = 0; it < ahead; ++it) {
-                if (rank == 0) mbar_expect_tx(full0 + it * 8, 2 * slot);             // of both CTAs
-                gi_tma_pair(ring0 + (uint32_t)it * slot, &map_w, it * 128, first / p.n_jobs * 256 + rank * 128, lead0 + it * 8);
-            }
-        __syncwarp();
-        if (p.early) pdl_wait();
+        if (p.early) {                                 // as above
+            if (elect_one())
+                for (int it = 0; it < min(GI_PREFETCH, nst); ++it) gi_prefetch(&map_w, it * 128, first / p.n_jobs * 256 + rank * 128);
+            __syncwarp();
+            pdl_wait();
+        }
         int s = 0; uint32_t ph = 1;
         for (int i = 0; i < n_items; ++i) {
             const int q = first + i * stride, tile = q / p.n_jobs, job = q - tile * p.n_jobs;
             for (int it = 0; it < nst; ++it) {
-                const bool there = i == 0 && it < ahead;
-                if (!there) mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
+                mbar_wait_spin(empty0 + s * 8, ph, p.status, 16);
                 if (elect_one()) {
                     const uint32_t bar = lead0 + s * 8, dst = ring0 + (uint32_t)s * slot;
-                    if (!there) {
-                        if (rank == 0) mbar_expect_tx(full0 + s * 8, 2 * slot);
-                        gi_tma_pair(dst, &map_w, it * 128, tile * 256 + rank * 128, bar);
-                    }
+                    if (rank == 0) mbar_expect_tx(full0 + s * 8, 2 * slot);          // of both CTAs
+                    gi_tma_pair(dst, &map_w, it * 128, tile * 256 + rank * 128, bar);
                     gi_tma_pair(dst + GI_A_BYTES, &map_x, it * 128, job * NT + rank * (NT / 2), bar);
                 }
                 __syncwarp();

@@ -28,7 +28,7 @@ constexpr size_t GV_SMEM = 64 * 1024, GV_SMEM_QUANTISED = 48 * 1024;
 struct GvParams {
     void* y; const int8_t* w; const float* sw; const void* x; const float* sx;
     size_t ldx, pitch;
-    int M, N, K, blocks, xpitch, units, batch, early;      // 64-k blocks of a row; bytes between activation rows in shared memory
+    int M, N, K, blocks, xpitch, units, batch;             // 64-k blocks of a row; bytes between activation rows in shared memory
 };
 
 enum { GV_X_F32 = B200_F32, GV_X_BF16 = B200_BF16, GV_X_I8 = B200_I8 };
@@ -165,19 +165,15 @@ k_gemv_i8(const __grid_constant__ GvParams p) {
     };
     uint4 wa[GV_LOADS], wb[GV_LOADS];
     // The first weights are asked into L2 while the kernel before still runs.  Nothing is read: L2 is where its writes go, too.
-    // 7.1 -> 6.4 us for one row x [4096 x 4096] in a row of calls; two units instead of one: 6.7.  (`early`: below.)
-    if (!p.early) {
-        const int n = (int)blockIdx.x * GV_ROWS + (lane & 7);
-        const int bytes = min((b1 - b0) * 64, (int)p.pitch - b0 * 64);
-        if (lane < 8 && n < p.N && bytes > 0)
-            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p.w + (size_t)n * p.pitch + b0 * 64), "r"(bytes) : "memory");
-    }
+    // 7.1 -> 6.4 us for one row x [4096 x 4096] in a row of calls; two units instead of one: 6.7.
+    const int ahead = (int)blockIdx.x * GV_ROWS + (lane & 7), bytes = min((b1 - b0) * 64, (int)p.pitch - b0 * 64);
+    if (lane < 8 && ahead < p.N && bytes > 0)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p.w + (size_t)ahead * p.pitch + b0 * 64), "r"(bytes) : "memory");
     // The scales of the units too, which are wanted last (one row x [4096 x 12288] 10.2 -> 9.95 us, [4096 x 4096] 5.1 -> 5.0).
     for (int i = tid; i < n_units; i += GV_THREADS)
         asm volatile("prefetch.global.L2 [%0];" :: "l"(p.sw + ((size_t)blockIdx.x + (size_t)i * gridDim.x) * GV_ROWS));
-    if (!p.early) pdl_wait();
+    pdl_wait();
     load(wa);
-    if (p.early) pdl_wait();                           // the activations' codes and scales
     gv_stage_x<XT>(p, xs, sxs, red, warp, lane);
     __syncthreads();
 
@@ -247,14 +243,13 @@ static size_t gv_x_bytes(int M, int K) { return (size_t)std::min(M + 1, 8) * gv_
 
 // Against the tensor-core kernel, codes x [4096 x 4096], us: 4 rows 5.3 and 7.2, 8 rows 6.2 and 7.2; [12288 x 4096] 10.8 and 13.7, 12.0 and
 // 13.8; but [154880 x 4096] 102.9 and 104.2, 108.8 and 104.9.
-bool gemv_i8_takes(int M, int N, int K, bool early) {
-    return M <= 8 && gv_x_bytes(M, K) <= (early ? GV_SMEM_QUANTISED : GV_SMEM) && (M <= 4 || (size_t)N * K <= ((size_t)1 << 28));
+bool gemv_i8_takes(int M, int N, int K, bool quantised) {
+    return M <= 8 && gv_x_bytes(M, K) <= (quantised ? GV_SMEM_QUANTISED : GV_SMEM) && (M <= 4 || (size_t)N * K <= ((size_t)1 << 28));
 }
 
 // x: M rows of x_dtype (B200_F32, B200_BF16 with ldx; B200_I8 with their scales sx).
-int gemv_i8(void* y, int y_bf16, const b200_i8_rows* W, const void* x, int x_dtype, size_t ldx, const float* sx, int M, int N, int K, int early, cudaStream_t s) {
+int gemv_i8(void* y, int y_bf16, const b200_i8_rows* W, const void* x, int x_dtype, size_t ldx, const float* sx, int M, int N, int K, cudaStream_t s) {
     GvParams p{};
-    p.early = early;
     p.y = y; p.w = W->q; p.sw = W->scale; p.x = x; p.sx = sx; p.ldx = ldx; p.pitch = i8_pitch(K);
     p.M = M; p.N = N; p.K = K;
     p.blocks = (K + 63) / 64;

@@ -32,7 +32,7 @@ k_i8_quantize(const void* xin, size_t ldx, int rows, int K, int8_t* q, float* sc
     __shared__ uint32_t red[I8Q_THREADS / 32];
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
     const size_t row = WARP ? (size_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x, pitch = i8_pitch(K);
-    // In this order: what starts now starts after all that came before this launch has ended (gemm_i8.cu relies on it).
+    // In this order: what starts now starts after all that came before this launch has ended (gemm_i8.cu takes its TMEM on that).
     pdl_wait();
     pdl_launch_dependents();
     if (WARP && row >= (size_t)rows) return;
@@ -180,7 +180,7 @@ extern "C" int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const v
     if (M > I8_MAX_ROWS || N > I8_MAX_ROWS || K > I8_MAX_K) return B200_ELIMIT;
     if (((uintptr_t)y & (y_dtype == B200_F32 ? 3 : 1)) || ((uintptr_t)W->q & 15) || ((uintptr_t)W->scale & 3)) return B200_EALIGN;
     b200_i8_rows xq;
-    const bool early = x_dtype != B200_I8;
+    const bool quantised = x_dtype != B200_I8;
     if (x_dtype == B200_I8) {
         xq = *static_cast<const b200_i8_rows*>(x);
         if (!xq.q || !xq.scale) return B200_EINVAL;
@@ -190,12 +190,12 @@ extern "C" int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const v
         if (!ws) return B200_EINVAL;
         if ((uintptr_t)ws & 255) return B200_EALIGN;
         if (gemv_i8_takes(M, N, K, false) && i8_gemv_quantises(M, K))
-            return gemv_i8(y, y_dtype == B200_BF16, W, x, x_dtype, ldx, nullptr, M, N, K, 0, stream);
+            return gemv_i8(y, y_dtype == B200_BF16, W, x, x_dtype, ldx, nullptr, M, N, K, stream);
         int8_t* q = static_cast<int8_t*>(ws);
         float* scale = reinterpret_cast<float*>(q + up256((size_t)M * i8_pitch(K)));
         if (int rc = i8_quantize_launch(x, x_dtype == B200_F32, ldx, M, K, q, scale, stream)) return rc;
         xq = b200_i8_rows{q, scale};
     }
-    if (gemv_i8_takes(M, N, K, early)) return gemv_i8(y, y_dtype == B200_BF16, W, xq.q, B200_I8, 0, xq.scale, M, N, K, early, stream);
-    return gemm_i8_wide(y, y_dtype == B200_BF16, W, &xq, M, N, K, early, stream);
+    if (gemv_i8_takes(M, N, K, quantised)) return gemv_i8(y, y_dtype == B200_BF16, W, xq.q, B200_I8, 0, xq.scale, M, N, K, stream);
+    return gemm_i8_wide(y, y_dtype == B200_BF16, W, &xq, M, N, K, quantised, stream);
 }

@@ -105,3 +105,24 @@ def test_binding_keeps_what_it_points_to(monkeypatch):
     for ws in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 20, dtype=torch.uint8)[::2], torch.zeros(100, dtype=torch.uint8)):
         with pytest.raises(P.B200Error, match='ws'):
             b.i8_gemm(W, x, ws=ws)
+
+
+def test_weights_are_read_behind_the_dependency_wait():
+    """Only the kernel's own griddepcontrol.wait makes an earlier kernel's writes visible, one that wrote the weights before the call's
+    quantiser too: the thread that asks for weights has waited by then, whatever the launch was told."""
+    import glob
+    import os
+    import re
+    import __graft_entry__ as G
+    source = lambda name: re.sub(r'//[^\n]*', '', open(os.path.join(G.PKG_DIR, 'csrc', name)).read())
+    kernels = re.split(r'\b__global__\b', source('gemm_i8.cu'))[1:]
+    assert len(kernels) == 2
+    for k in kernels:
+        start = re.search(r'if \(!p\.early\) pdl_wait\(\);', k)
+        loader = k[k.index('if (warp == 0) {'):]
+        first = re.search(r'(gx_tma_2d|gi_tma_pair)\([^;]*map_w', loader)
+        waited = re.search(r'if \(p\.early\) \{(?:[^{}]|\{[^{}]*\})*pdl_wait\(\);\s*\}', loader)
+        assert start and first and waited and waited.end() < first.start()
+    gemv = re.split(r'\b__global__\b', source('gemv_i8.cu'))[1]
+    wait, first = re.search(r'^    pdl_wait\(\);', gemv, re.M), re.search(r'^ *(if \(.*\) )?load\(wa\);', gemv, re.M)
+    assert wait and first and wait.end() < first.start()
