@@ -135,7 +135,8 @@ template <int XT, bool BF16>
 __global__ void __launch_bounds__(GV_THREADS, 2)
 k_gemv_i8(const __grid_constant__ GvParams p) {
     extern __shared__ __align__(16) int8_t xs[];       // [M][xpitch]
-    __shared__ int part[GV_PART];                      // [unit of the batch][warp][token][8 rows]
+    __shared__ __align__(16) int part[GV_PART];        // [unit of the batch][warp][token][8 rows]
+    static_assert(__alignof__(part) >= alignof(int2), "partial sums are stored in pairs");
     __shared__ float sxs[8];
     __shared__ uint32_t red[GV_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
