@@ -85,6 +85,20 @@ def test_against_the_formula(M, V, top, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('M,V,top', [(593, 32768, 5), (600, 1000, 32), (700, 20011, 20), (1200, 77, 0), (900, 4099, 1), (640, 2048, 8), (2000, 33, 32)])
+def test_many_rows(M, V, top, dtype):
+    """Rows enough for the smallest blocks, whole and under masks that leave a row little or nothing.  A thread of 128 adds V / 256 terms to
+    each of its two sums, 128 at most, where `check` allows for V / 512 + 164."""
+    x, t = make(M, V, M + V, dtype)
+    check(x, t, top)
+    g = torch.Generator().manual_seed(V)
+    x[torch.rand((M, V), generator=g) < 0.97] = -INF
+    x[1], x[2], x[3, V // 2], x[4, V - 1] = -INF, torch.finfo(dtype).min, float('nan'), INF
+    x[M - 1] = 2.5
+    check(x, t, top)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('off,pad', [(0, 0), (1, 0), (3, 5), (2, 1), (5, 3), (8, 47)])
 def test_strides_and_alignments(dtype, off, pad):
     M, V = 11, 20011
