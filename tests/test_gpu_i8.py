@@ -165,6 +165,57 @@ def test_product_is_exact(M, N, K):
     assert P.device_status() == 0
 
 
+# On 148 multiprocessors these go to pairs of CTAs, in tiles of 64, 96, 128, 160, 160, 192, 192, 224, 224, 256 and 256 tokens; one, two or three
+# items a pair (up to 20, 28, 114, 50, 200, 50, 190, 50, 180, 50 and 180 items for 74 pairs).
+PAIRS = [(289, 1010, 1029), (644, 1001, 1029), (338, 9523, 1300), (290, 6310, 1029), (580, 12576, 1029), (323, 6356, 1029), (808, 9505, 1029),
+         (417, 6342, 771), (840, 11268, 771), (453, 6359, 771), (897, 11280, 771)]
+
+
+@pytest.mark.parametrize('M,N,K', PAIRS)
+def test_product_on_pairs_is_exact(M, N, K):
+    P = pkg()
+    i = PAIRS.index((M, N, K))
+    x, w = inputs(M, N, K, 100 + i, (torch.float32, torch.bfloat16)[i & 1])
+    want = product(*rows_of(x), *rows_of(w), torch.float32)
+    W, X = P.i8_quantize(w.cuda()), P.i8_quantize(x.cuda())
+    for dtype in (torch.float32, torch.bfloat16):
+        buf = torch.full((M * N + 999,), 3.0, dtype=dtype, device='cuda')
+        P.i8_gemm(W, x.cuda(), buf[:M * N].view(M, N))
+        assert same(buf[:M * N].view(M, N), want.to(dtype)) and (buf[M * N:] == 3).all()
+        assert same(P.i8_gemm(W, X, dtype=dtype), want.to(dtype))
+    assert P.device_status() == 0
+
+
+# Up to 8 rows: a warp's slice of K in several turns of loads (K above 4096, the last turn part full), and more units of weight rows to a CTA than
+# its partial sums have room for at once (64 / M).
+@pytest.mark.parametrize('M,N,K', [(1, 301, 4097), (1, 4100, 5003), (1, 77, 8192), (1, 300, 12288), (2, 200, 8200), (1, 130, 30000), (2, 97, 20001), (3, 500, 12289),
+                                   (4, 64, 12288), (8, 160, 6200), (1, 160001, 192), (2, 154880, 256), (3, 50021, 100), (5, 60007, 300), (7, 43001, 129),
+                                   (8, 40001, 520), (8, 20000, 4500)])
+def test_few_rows_with_long_sums_and_many_outputs(M, N, K):
+    P = pkg()
+    x, w = inputs(M, N, K, M + N + K, (torch.float32, torch.bfloat16)[K & 1])
+    want = product(*rows_of(x), *rows_of(w), torch.float32)
+    W, X = P.i8_quantize(w.cuda()), P.i8_quantize(x.cuda())
+    for dtype in (torch.float32, torch.bfloat16):
+        assert same(P.i8_gemm(W, x.cuda(), dtype=dtype), want.to(dtype))
+        assert same(P.i8_gemm(W, X, dtype=dtype), want.to(dtype))
+
+
+def test_few_rows_with_weights_past_32_bits():
+    """More than 2^31 bytes of weights in the kernel of few rows: one row quantised in the kernel, and finished rows."""
+    P = pkg()
+    N, K = 180001, 12288
+    g = torch.Generator(device='cuda').manual_seed(2)
+    q = torch.randint(-127, 128, (N, K), generator=g, device='cuda', dtype=torch.int8)
+    sw = torch.rand(N, generator=g, device='cuda')
+    W = P.I8Rows(q, sw, K)
+    for M in (1, 2):
+        x = torch.randn((M, K), generator=g, device='cuda')
+        y = P.i8_gemm(W, x if M == 1 else P.i8_quantize(x)).cpu()
+        for a in (0, N // 2, N - 200):
+            assert same(y[:, a:a + 200].contiguous(), product(*rows_of(x.cpu()), q[a:a + 200].cpu().numpy(), sw[a:a + 200].cpu().numpy(), torch.float32))
+
+
 @pytest.mark.parametrize('M', [1, 4, 20, 150, 520])
 def test_largest_sums(M):
     """Codes of the caller's own, -128 among them, at the longest K: sums up to 2^30."""
