@@ -20,10 +20,12 @@ constexpr int GV_WARPS = 8, GV_THREADS = GV_WARPS * 32, GV_ROWS = 8;
 constexpr int GV_LOADS = 8;                        // 64-k blocks a warp loads at once
 constexpr int GV_KEEP = 2;                         // vectors of 8 activations a thread keeps between maximum and codes
 constexpr int GV_PART = 4096;                      // partial sums of a batch of units
-// Activations of a CTA, in bytes of shared memory.  Every CTA brings all of them: codes x [4096 x 12288], 4 rows (60 KB) 12.2 us, 6 rows
-// (84 KB) 21.3, where gemm_i8.cu takes 14.1.  Behind the quantiser, whose end they have to wait for, 2 rows (36 KB) 14.1, 3 rows
-// (48 KB) 15.0, 4 rows 16.3, and 14.9 there.
-constexpr size_t GV_SMEM = 64 * 1024, GV_SMEM_QUANTISED = 48 * 1024;
+// Activations of a CTA, in bytes of shared memory, at most: every CTA brings all of them.  us here and in gemm_i8.cu, on finished rows: 8 rows
+// (33 KB) x [4096 x 4096] 7.0 and 6.8, x [2000 x 4096] 4.7 and 6.0, 4 rows (33 KB) x [1000 x 6500] 5.4 and 5.7, but 8 rows (42 KB) x [4096 x 5120] 8.8 and
+// 7.5, 4 rows (60 KB) x [4096 x 12288] 13.3 and 12.0; 2 rows (37 KB) x [4096 x 12288] 10.7 and 11.9, (43 KB) x [4096 x 14336] 13.7 and 13.3.  Behind
+// the quantiser, whose end they have to wait for: 4 rows (21 KB) x [4096 x 4096] 8.0 and 8.4, x [12288 x 4096] 12.4 and 12.7, but 5 rows (25 KB) 8.5 and
+// 8.4, 13.0 and 12.7, 8 rows (33 KB) 9.4 and 8.4, 14.1 and 12.8; 2 rows (37 KB) x [4096 x 12288] 12.9 and 13.8, 1 row (47 KB) x [4096 x 24000] 23.4 and 25.8.
+constexpr size_t GV_SMEM = 34 * 1024, GV_SMEM_QUANTISED = 24 * 1024, GV_SMEM_2 = 38 * 1024, GV_SMEM_2_QUANTISED = 48 * 1024, GV_SMEM_MAX = 48 * 1024;
 
 struct GvParams {
     void* y; const int8_t* w; const float* sw; const void* x; const float* sx;
@@ -227,7 +229,7 @@ static int gv_launch(const GvParams& p, size_t smem, cudaStream_t s) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return launch_failed("gemv_i8: cudaGetDevice");
     if (dev < 0 || dev >= 64 || !ready[dev]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GV_SMEM) != cudaSuccess)
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GV_SMEM_MAX) != cudaSuccess)
             return launch_failed("gemv_i8: cudaFuncSetAttribute");
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
@@ -242,10 +244,11 @@ static int gv_xpitch(int K) {
 // The rows, one of zeros, and what the last chunk of a slice may read past the end (and multiplies by zero).
 static size_t gv_x_bytes(int M, int K) { return (size_t)std::min(M + 1, 8) * gv_xpitch(K) + GV_LOADS * 64; }
 
-// Against the tensor-core kernel, codes x [4096 x 4096], us: 4 rows 5.3 and 7.2, 8 rows 6.2 and 7.2; [12288 x 4096] 10.8 and 13.7, 12.0 and
-// 13.8; but [154880 x 4096] 102.9 and 104.2, 108.8 and 104.9.
+// Five and more rows of a matrix that fills the GPU many times over are the tensor-core kernel's: 8 rows x [154880 x 2048] 77.3 us here and 53.3 there,
+// x [154880 x 4096] 100.0 and 100.5 (5 rows 96.3 and 99.3); 4 rows 93.6 and 99.8, 8 rows x [40000 x 4096] 28.0 and 32.4.
 bool gemv_i8_takes(int M, int N, int K, bool quantised) {
-    return M <= 8 && gv_x_bytes(M, K) <= (quantised ? GV_SMEM_QUANTISED : GV_SMEM) && (M <= 4 || (size_t)N * K <= ((size_t)1 << 28));
+    const size_t most = M <= 2 ? (quantised ? GV_SMEM_2_QUANTISED : GV_SMEM_2) : quantised ? GV_SMEM_QUANTISED : GV_SMEM;
+    return M <= 8 && gv_x_bytes(M, K) <= most && (M <= 4 || (size_t)N * K <= ((size_t)1 << 28));
 }
 
 // x: M rows of x_dtype (B200_F32, B200_BF16 with ldx; B200_I8 with their scales sx).

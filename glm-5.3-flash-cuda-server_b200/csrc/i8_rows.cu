@@ -142,8 +142,8 @@ int i8_quantize_launch(const void* x, int x_is_f32, size_t ldx, int rows, int K,
 
 // Up to so many activations the few-row kernel quantises them itself, in every CTA; beyond, in a launch of its own.  us with either in
 // replays (and for calls from the host, where a launch costs more), bf16: 1 row x [4096 x 4096] 5.9 and 6.8 (6.1 and 8.0), x [4096 x 12288]
-// 11.8 and 12.2, x [4096 x 16384] 16.8 and 15.8; 2 rows x [4096 x 4096] 6.8 and 7.2, x [4096 x 8192] 10.5 and 10.3; 3 rows x [4096 x 4096] 8.5 and
-// 7.5 (8.7 and 8.3); 4 rows x [4096 x 2048] 5.9 and 6.2; 5 rows x [4096 x 1600] 6.8 and 6.2 (7.1 and 7.9).
+// 11.9 and 12.2, x [4096 x 16384] 16.6 and 14.7; 2 rows x [4096 x 4096] 6.9 and 7.0, x [4096 x 8192] 10.4 and 10.0; 3 rows x [4096 x 4096] 8.5 and
+// 7.6 (8.7 and 8.3); 4 rows x [4096 x 2048] 5.9 and 6.3; 5 rows x [4096 x 1600] 6.8 and 6.3 (7.1 and 7.9).
 static bool i8_gemv_quantises(int M, int K) { return (size_t)M * K <= (M == 1 ? 12288 : 8192); }
 
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }

@@ -190,7 +190,8 @@ def test_product_on_pairs_is_exact(M, N, K):
 # its partial sums have room for at once (64 / M).
 @pytest.mark.parametrize('M,N,K', [(1, 301, 4097), (1, 4100, 5003), (1, 77, 8192), (1, 300, 12288), (2, 200, 8200), (1, 130, 30000), (2, 97, 20001), (3, 500, 12289),
                                    (4, 64, 12288), (8, 160, 6200), (1, 160001, 192), (2, 154880, 256), (3, 50021, 100), (5, 60007, 300), (7, 43001, 129),
-                                   (8, 40001, 520), (8, 20000, 4500)])
+                                   (8, 40001, 520), (8, 20000, 4500),
+                                   (2, 300, 12288), (1, 130, 18000), (1, 130, 24000), (4, 300, 6500), (3, 70, 8000), (8, 50, 4095)])
 def test_few_rows_with_long_sums_and_many_outputs(M, N, K):
     P = pkg()
     x, w = inputs(M, N, K, M + N + K, (torch.float32, torch.bfloat16)[K & 1])
