@@ -18,9 +18,11 @@
 // dependency wait, the weights neither: only that wait makes an earlier kernel's writes visible.
 // Rows past N or M and columns past K come as zero from the tensor maps.  Every wait is bounded (tma_pipe.cuh).
 //
-// Bound by what an SM takes in from L2 (about 43 bytes per clock, 82 GB/s) where the tiles are few, by the weights' stream from HBM where
-// the tokens are (24 rows x [4096 x 12288] 13.9 us, of which 8.9 are the stream at 5.7 TB/s), by the matrix instructions and the power that
-// they draw at 2048 rows ([12288 x 4096] 70 us, 2.94 POP/s, in a short run; 82 us in a long one, where zeros as operands still take 62).
+// Bound by what an SM takes in: between the first and the last step of an item 50 to 70 bytes a clock (time stamps; 301 rows x [8192 x 4096], whose
+// weights come out of L2 for the second tile of tokens, 70; 150 x [12288 x 4096] 60), where pairs with 256 tokens a tile need 64 to keep the matrix
+// instructions busy.  Few tokens are bound by the weights' stream from HBM (24 rows x [4096 x 12288] on finished rows 12.5 us: 7.0 from the first
+// step to the last, 2.5 for the two cluster barriers and the sums), 2048 rows by the matrix instructions and the power that they draw ([12288 x 4096]
+// on finished rows 71 us, 2.91 POP/s, in a short run; with the quantiser 75, and 89 in a long run).
 #include "b200_internal.h"
 #include "umma_mxf4.cuh"
 #include <cuda.h>
@@ -441,12 +443,13 @@ static int gi_launch(GiParams& p, const b200_i8_rows* W, const b200_i8_rows* x, 
 
 // Which kernel, and how many tokens per tile: what takes the fewest clocks by this estimate.  A step of 128 k is 2 NT clocks of MMA, or
 // as long as an SM takes to bring its part of the tile at 60 B per clock; what an item has besides is about 1000 clocks, 2500 for a
-// pair, and where CTAs share it also the sums that they pass on (these three fitted to the shapes below and some twenty more).
-//   shared   as many CTAs share an item as one per SM leaves room for: 24 rows x [4096 x 12288], 32 items, 27.2 us with one, 18.0, 14.6
-//            and 13.3 with 2, 3 and 4; but on the SMs' second places they lose (16 rows x [12288 x 4096], 96 items, 12.4 with one, 14.0 with 2)
-//   tiles    777 rows x [5003 x 2048], in pairs: four tiles of 224 tokens are 80 items for 74 pairs, 16.8 us, seven of 128 are 140, 13.5
-//   pairs    2048 rows x [12288 x 4096] 80.6 us with single CTAs, 70.0 in pairs; 301 x [8192 x 4096] 15.4 and 14.3; but 48 x [12288 x
-//            4096] 13.8 and 14.2; 250 x [2000 x 4096] 9.0 shared, 11.0 in pairs; 600 x [1000 x 2000] 12.0 shared, 8.7 in pairs
+// pair, and where CTAs share it also the sums that they pass on (these three fitted to the shapes below and some twenty more; 44 B per clock
+// chose worse on 200 x [4096 x 4096], 600 x [1000 x 2000] and 300 x [6000 x 1500]).  us on finished rows:
+//   shared   as many CTAs share an item as one per SM leaves room for: 24 rows x [4096 x 12288], 32 items, 22.9 with one, 16.4, 13.7
+//            and 12.5 with 2, 3 and 4; but on the SMs' second places they lose (16 rows x [12288 x 4096], 96 items, 11.5 with one, 13.1 with 2)
+//   tiles    777 rows x [5003 x 2048], in pairs: four tiles of 224 tokens are 80 items for 74 pairs, 16.8, seven of 128 are 140, 13.2
+//   pairs    2048 rows x [12288 x 4096] 82 with single CTAs, 71 in pairs; 301 x [8192 x 4096] 15.6 and 12.6; but 48 x [12288 x 4096]
+//            11.9 and 11.9; 250 x [2000 x 4096] 9.6 shared, 10.0 in pairs; 600 x [1000 x 2000] 6.7 with single CTAs, 7.0 in pairs, 9.2 shared
 struct GiPlan { int M, N, K, pair, NT, n_jobs, total, split; };
 static GiPlan gi_plan(int M, int N, int K) {
     GiPlan g{M, N, K, 0, 0, 0, 0, 1};

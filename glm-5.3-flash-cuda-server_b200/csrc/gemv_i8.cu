@@ -8,7 +8,8 @@
 //   units of 8 weight rows; a CTA of 8 warps takes every gridDim-th unit, warp w the w-th slice of K of each; partial sums go to
 //   shared memory, whole numbers, so that their order does not matter; after a batch of units the CTA adds and writes them.
 //   A warp has the next 8 loads (4 KB) in flight while it multiplies the present ones.
-// One row x [154880 x 4096] 97 us (6.5 TB/s), [12288 x 4096] 10.5 us, [4096 x 4096] 5.8 us with about 3.5 us that no byte costs.  What
+// One row, quantised in the kernel, in replays: x [154880 x 4096] 92 us (6.9 TB/s: reads alone exceed the rate of a copy), [12288 x 4096] 10.5 us,
+// [4096 x 4096] 5.9 us (5.2 with the weights in L2), about 3.5 of them the start, the row's codes and the last sums, which no byte costs.  What
 // mattered is the number of instructions: with a test and a copy for every load 52 per 512 bytes of weights instead of 23, and 112 us.
 #include "b200_internal.h"
 #include "tma_pipe.cuh"

@@ -14,16 +14,19 @@
 // fma(x, log2 e, -fl(m log2 e)): its distance from (x - m) log2 e is the same for every element and corrected when m changes.
 //
 // The likeliest tokens.  Order: logit descending, then index ascending, as one 64-bit key.  A bound is a value that at least `top`
-// elements reach: the top-th of the two largest maxima of every warp.  The first tile gives one, and later elements count only
+// elements reach: the top-th of the largest maxima of every warp, 32 in all.  The first tile gives one, and later elements count only
 // above it (an equal one has a larger index).  Vectors whose maximum counts go to a list in shared memory, and after 1, 4, 16, ...
 // tiles the list gives a higher bound: some 200 vectors of a vocabulary of 154880 in no particular order.  In the end the elements
 // of these vectors that reach the last bound, little more than `top`, are put in order by counting who is larger.  A list that
 // overflows (logits in ascending order; a first tile of masked tokens before thousands of others) is dropped, and the CTA
 // finds the top-th key by radix selection over its part instead.
 //
-// [2048 x 154880] f32 185 us (6.9 TB/s), with 20 alternatives 218; bf16 128 and 172, where the exponential bounds it: 16 a clock and SM are
-// 75 us, and the instructions of an element, about 10 in all, not much less.  [512 x 154880] bf16 42.5 us: 512 rows on 148 SMs are 4 rows
-// on some and 3 on others.  One row of 154880, top 5, 9 us, none of them a unit's limit: a chain of loads, barriers and exchanges.
+// In replays: [2048 x 154880] f32 186 us (6.8 TB/s: reads alone exceed the rate of a copy), with 20 alternatives 214; bf16 126 and 169, where the
+// exponential bounds the sums (16 a clock and SM are 75 us; the instructions of an element, about 10 in all, take not much less) and the top costs
+// bounds and lists for which the stream waits at a row's two ends.  A long run of calls on f32 rows with 20
+// alternatives takes 234 us a call.
+// [512 x 154880] bf16 42 us: 512 rows on 148 SMs are 4 rows on some and 3 on others.  One row of 154880, top 5, 9.0 us, none of them a unit's limit: a
+// chain of loads, barriers and exchanges.
 #include "b200_internal.h"
 #include "tma_pipe.cuh"
 #include <cuda_bf16.h>
@@ -84,8 +87,8 @@ __device__ __forceinline__ LpStat lp_join(LpStat a) {
     return LpStat{m, a.n, a.s, a.t};
 }
 
-// A bound: the top-th of the largest two (four) k of every one of 16 (8) warps, 0 if there are not so many.  Every thread calls it and gets
-// it.
+// A bound: the top-th of the largest two (four, eight) k of every one of 16 (8, 4) warps, 0 if there are not so many.  Every thread calls it and
+// gets it.
 template <int LP_THREADS>
 __device__ __noinline__ uint32_t lp_bound(uint32_t k, int top) {
     __shared__ uint32_t w[32];
@@ -582,10 +585,11 @@ static int lp_choose(const LpParams& p, int M, cudaStream_t s) {
     // CTAs per row: as many as leave the whole batch on the GPU at once (two CTAs per SM), and a tile's worth of work to each.
     int C = LP_CLUSTER;
     while (C > 1 && ((long long)M * C > 2 * sm_count() || p.V / C < 512 * LP_VECS * LpVec<F32>::N)) C >>= 1;
-    // Threads per CTA (1024 per SM in any case): few large CTAs where a row's time counts, small ones, whose barriers cost the others
-    // nothing, where there are rows enough.  us with 512 / 256 / 128: [1 x 154880] f32, top 5 10.8 / 12.8 / 17.6; [200 x 20000] f32,
-    // top 20 14.4 / 16.4 / 23.3; [300 x 1000] f32, top 5 12.1 / 6.9 / 7.4; [2048 x 154880] f32, top 20 227 / 222 / 234, bf16
-    // 194 / 177 / 172; [2000 x 20000] bf16, top 20 71 / 62 / 56; [2000 x 600] bf16, top 5 54 / 34 / 22.
+    // Threads per CTA: few large CTAs where a row's time counts, small ones, whose barriers cost the others nothing, where there are rows enough.
+    // 12 KB of an SM's shared memory go to each CTA besides its ring (and 1 KB to the system), so two of 512 threads have room on it, three of 256
+    // or six of 128; the launch bounds hold each form to 64 registers, which only the first needs.  us with 512 / 256 / 128: [1 x 154880] f32,
+    // top 5 9.2 / 11.7 / 16.1; [200 x 20000] f32, top 20 11.7 / 15.0 / 21.9; [300 x 1000] f32, top 5 11.7 / 6.8 / 7.2; [2048 x 154880] f32, top 20
+    // 223 / 214 / 236, bf16 181 / 170 / 167; [2000 x 20000] bf16, top 20 69.7 / 54.4 / 54.3; [2000 x 600] bf16, top 5 53.3 / 33.6 / 21.3.
     const size_t vecs = (size_t)p.V / LpVec<F32>::N;
     if (M > 4 * sm_count()) return vecs <= 8192 ? lp_launch<F32, 128>(p, M, C, s) : lp_launch<F32, 256>(p, M, C, s);
     return C == 1 && vecs <= 1024 ? lp_launch<F32, 256>(p, M, C, s) : lp_launch<F32, 512>(p, M, C, s);

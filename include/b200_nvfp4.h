@@ -231,7 +231,7 @@ typedef struct {
 size_t b200_i8_pitch(int K);
 
 /* x [rows, K] (dtype B200_F32 or B200_BF16, rows ldx >= K elements apart, at its type's alignment; 16-byte aligned rows are
- * fastest) -> q, scale.  K <= 65536, rows <= 2^24 (B200_ELIMIT). */
+ * fastest) -> q, scale, which may overlap neither each other nor x.  K <= 65536, rows <= 2^24 (B200_ELIMIT). */
 int b200_i8_quantize(const void* x, int dtype, size_t ldx, int rows, int K, int8_t* q, float* scale, b200_stream stream);
 
 /* y[m, n] = x_scale[m] * W.scale[n] * sum_k xq[m, k] * W.q[n, k], y [M, N] row-major f32 (y_dtype B200_F32) or bf16.
@@ -257,7 +257,7 @@ int b200_i8_gemm(void* y, int y_dtype, const b200_i8_rows* W, const void* x, int
  * Masked tokens have logit -inf (ln p = -inf) or the type's lowest value.  A row of -inf alone has no distribution: its log
  * probabilities are -inf, its entropy 0, its ids the lowest.  A row that holds +inf or a NaN: NaN, and ids of -1 (a negative
  * token still gives 0).  Sums are held in f32, and the likeliest token's share apart from the others', so that ln p of a nearly certain token keeps its
- * relative precision.  The same call gives the same bits.  No workspace.  V <= 2^30, M <= 2^24 (B200_ELIMIT).
+ * relative precision.  The same call gives the same bits.  Outputs may not overlap the inputs.  No workspace.  V <= 2^30, M <= 2^24 (B200_ELIMIT).
  * The reference copies the logits to the host for each token (src/engine.cu:706) and has no counterpart. */
 enum { B200_LOGPROBS_TOP_MAX = 32 };
 int b200_token_logprobs(const void* logits, int dtype, size_t ld, int M, int V, const int32_t* tokens, int G, float* logprobs,
