@@ -75,3 +75,32 @@ def test_a_layer_s_first_call_is_on_another_stream(M):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert P.device_status() == 0
+
+
+def test_calls_on_a_side_stream_of_a_captured_graph():
+    """A captured graph forks, calls on the side stream with outputs and scratch of their own, and joins; replayed on new inputs."""
+    P = pkg()
+    g = torch.Generator(device='cuda').manual_seed(5)
+    w = (torch.randn((700, 1024), generator=g, device='cuda') * 0.02).to(torch.bfloat16)
+    W, Wn = P.i8_quantize(w), weight(P, 512, 1024, 5)
+    x = torch.randn((40, 1024), generator=g, device='cuda')
+    t = torch.zeros((40, 1), dtype=torch.int32, device='cuda')
+
+    def calls(s):
+        y = P.i8_gemm(W, x, stream=s)
+        return [y, P.i8_gemm(W, P.i8_quantize(x, stream=s), stream=s), *P.token_logprobs(y, t, 4, stream=s), P.gemm(Wn, x[:8], stream=s)]
+
+    calls(None)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        got = calls(side)
+        torch.cuda.current_stream().wait_stream(side)
+    for seed in (6, 7):
+        x.copy_(torch.randn((40, 1024), generator=g.manual_seed(seed), device='cuda'))
+        graph.replay()
+        other = [torch.full((1 << 16,), 7.0, device='cuda') for _ in range(4)]            # memory that is not the graph's
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, calls(None)))
+        del other
