@@ -96,7 +96,7 @@ extern "C" const char* b200_nvfp4_strerror(int code) {
         case B200_OK: return "ok";
         case B200_EINVAL: return "invalid argument";
         case B200_ESHAPE: return "unsupported shape (K must be a multiple of 16)";
-        case B200_EALIGN: return "pointer not 4-byte aligned";
+        case B200_EALIGN: return "pointer not aligned as the call asks";
         case B200_ELAUNCH: return "CUDA launch failed";
         case B200_ELIMIT: return "size beyond the documented maximum";
         case B200_ENOTIMPL: return "not implemented";

@@ -126,3 +126,10 @@ def test_weights_are_read_behind_the_dependency_wait():
     gemv = re.split(r'\b__global__\b', source('gemv_i8.cu'))[1]
     wait, first = re.search(r'^    pdl_wait\(\);', gemv, re.M), re.search(r'^ *(if \(.*\) )?load\(wa\);', gemv, re.M)
     assert wait and first and wait.end() < first.start()
+
+
+def test_the_message_of_a_misaligned_pointer_holds_for_every_call():
+    """Codes want 16 bytes, scratch 256: the message of B200_EALIGN names no number."""
+    import re
+    L = pkg().lib()
+    assert 'align' in L.b200_nvfp4_strerror(EALIGN).decode() and not re.search(r'\d', L.b200_nvfp4_strerror(EALIGN).decode())
