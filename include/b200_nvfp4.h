@@ -31,7 +31,7 @@ enum {
     B200_OK = 0,
     B200_EINVAL = 1,      /* null pointer, non-positive size, M out of range */
     B200_ESHAPE = 2,      /* K not a multiple of 16, or a shape the kernel cannot tile */
-    B200_EALIGN = 3,      /* pointer below the 4-byte floor the format guarantees */
+    B200_EALIGN = 3,      /* pointer not aligned as the call asks (NVFP4: the 4-byte floor the format guarantees) */
     B200_ELAUNCH = 4,     /* the CUDA runtime refused the launch (cudaGetLastError text logged) */
     B200_ELIMIT = 5,      /* size beyond a documented maximum */
     B200_ENOTIMPL = 6,
